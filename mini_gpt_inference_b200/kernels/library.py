@@ -102,6 +102,11 @@ _SIGNATURES = {
                                  _F, _I, _I, _P, _P],
     "mg_attention_prefill_tc": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I,
                                 ctypes.c_longlong, _I, _I, _F, _I, _I, _P, _I, _P, _P],
+    "mg_attention_shared": [_P, ctypes.c_longlong, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I,
+                            _F, _I, _P],
+    "mg_beam_select": [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, ctypes.c_double, _P, _P, _P, _P, _P, _P, _P, _P],
+    "mg_beam_reorder": [_P, _P, _P, _I, _I, _P, _P, _P, _P, _I, _P, _P, _P, _P],
+    "mg_step_tables": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P],
     "mg_copy_ints": [_P, _P, _I, _P],
     "mg_argmax": [_P, _P, _I, _I, _I, _P],
     "mg_argmax_wide": [_P, _P, _P, _P, _I, _I, _I, _P],
@@ -116,7 +121,7 @@ _SIGNATURES = {
 # exported readers of the kernel files' index guards: mg_<name>_index_fault(long long[4])
 GUARDED_FILES = ("elementwise", "linear_skinny", "linear_stream", "linear_wide", "linear_cluster", "linear_tc",
                  "attention_generic", "attention_fp32", "attention_split", "attention_prefill", "head_prepare", "moe", "moe_few", "attention_mma", "matrix_memory", "matrix_memory_chunked",
-                 "rotary_prepare", "short_conv", "recurrent_gate", "residual_norm")
+                 "rotary_prepare", "short_conv", "recurrent_gate", "residual_norm", "attention_shared", "beam", "step_tables")
 for _name in GUARDED_FILES:
     _SIGNATURES[f"mg_{_name}_index_fault"] = [_P]
 GUARD_CODES = {1: "token id", 2: "position", 3: "cache row", 4: "page", 5: "request", 6: "row", 7: "token source"}
@@ -168,6 +173,10 @@ def load(verbose: bool = True):
     lib.mg_attention_mma_scratch_floats.restype = ctypes.c_longlong
     lib.mg_attention_split_scratch_floats.argtypes = [c_int, c_int, c_int, c_int]
     lib.mg_attention_split_scratch_floats.restype = ctypes.c_longlong
+    lib.mg_attention_shared_scratch_floats.argtypes = [c_int] * 8
+    lib.mg_attention_shared_scratch_floats.restype = ctypes.c_longlong
+    lib.mg_beam_select_scratch_bytes.argtypes = [c_int] * 4
+    lib.mg_beam_select_scratch_bytes.restype = ctypes.c_longlong
     _lib = lib
     return lib
 

@@ -9,7 +9,9 @@ computes anything on this path.
 from __future__ import annotations
 
 import ctypes
+import math
 import weakref
+from dataclasses import dataclass
 
 import torch
 
@@ -20,6 +22,7 @@ from .library import KernelLibraryError, check
 EPILOGUES = {"none": 0, "gelu_tanh": 1, "residual": 2, "relu_sq": 3}
 PLAIN_ACTIVATIONS = {"relu_sq": 0, "gelu_tanh": 1, "silu": 2}           # ... and the activation of a unit without a gate
 GATED_ACTIVATIONS = {"silu": 0, "clamped_swish": 1, "gelu_tanh": 2}     # the gated product of a unit's two halves
+MAX_BEAMS = 32           # most beams of a group in a search
 MOE_TC_EXPERTS = 256     # most experts the tensor-core tiles take
 MOE_FEW_TOKENS = 16      # most tokens the experts' kernels for few tokens take
 # More tokens than this take the heads' small products on the tensor-core GEMM.  (us, mma.sync / tcgen05: 16 heads of 128 -> 512
@@ -76,11 +79,39 @@ class EntrySum:
         self.shape = (entry_slot.shape[0], terms.shape[1])
 
 
+@dataclass
+class BeamChoice:
+    """What ``beam_select`` chose, one entry per row of the next step (``groups * beams``; ``scores`` as ``[groups, beams]``).
+    ``parents``: the row that each row's beam goes on from; ``ranks``: its place among its group's, 0 the best."""
+
+    tokens: torch.Tensor
+    parents: torch.Tensor
+    scores: torch.Tensor
+    ranks: torch.Tensor
+    ended: torch.Tensor | None = None
+    lengths: torch.Tensor | None = None
+
+
+@dataclass
+class StepTables:
+    """A step's integers as ``step_tables`` leaves them on the device (see ``StepContext`` for what each is)."""
+
+    token_request: torch.Tensor
+    positions: torch.Tensor
+    req_q_start: torch.Tensor
+    block_tables: list
+    slot_mapping: list
+
+
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
+
+
+def _pointers(tensors):
+    return (ctypes.c_void_p * len(tensors))(*(_ptr(t) for t in tensors))
 
 
 class CudaOps:
@@ -859,6 +890,9 @@ class CudaOps:
             plan.signature.append(("attention_merge", batch.max_ctx_after > KEY_CHUNK))
 
     def paged_attention(self, qkv, n_head, n_kv_head, head_dim, scale, cache, ctx):
+        if getattr(ctx, "shared_prefix", None) is not None and not cache.window and head_dim <= 256:
+            # rows that have their first tokens in common: those keys are read once for a group
+            return self.paged_attention_shared(qkv, n_head, n_kv_head, head_dim, scale, cache, ctx)
         self._want(qkv, cache.k_pages.dtype, "qkv", 2)
         table = self._want(ctx.block_tables[cache.group], torch.int32, "block_table", 2)
         n = qkv.shape[0]
@@ -924,6 +958,43 @@ class CudaOps:
             _ptr(ctx.token_request), _ptr(ctx.positions), _ptr(out), n, n_head, n_kv_head, head_dim,
             cache.page_tokens, table.shape[1], window, float(scale), cache.k_pages.shape[0], table.shape[0],
             self._is_bf16(qkv), self._stream()), "paged_attention")
+        return out
+
+    def paged_attention_shared(self, qkv, n_head, n_kv_head, head_dim, scale, cache, ctx):
+        """``paged_attention`` for a step of single tokens, groups of which share their first tokens
+        (``ctx.shared_prefix``, see ``SharedPrefix``): a group's common keys and values are read once.  Each row sees the
+        keys 0 .. its position of its own request; a row in front of the end of its group's shared tokens, or of no group,
+        reads all of them for itself; one at a position below zero is padding, its result zeros.  Heads of up to 256
+        features; no window, no values in the key rows."""
+        shared = ctx.shared_prefix
+        k, v, n = cache.k_pages, cache.v_pages, qkv.shape[0]
+        self._want(qkv, k.dtype, "qkv", 2)
+        is_bf16 = self._is_bf16(qkv)
+        table = self._want(ctx.block_tables[cache.group], torch.int32, "block_table", 2)
+        groups = self._want(shared.groups, torch.int32, "groups of rows", 2)
+        if self._want(v, k.dtype, "v_pages", 4).shape != self._want(k, None, "k_pages", 4).shape or (
+                tuple(k.shape[1:]) != (n_kv_head, cache.page_tokens, head_dim)):
+            raise KernelLibraryError("attention (shared): page storage does not match the head sizes")
+        if cache.window or getattr(cache, "values_in_keys", False):
+            raise KernelLibraryError("attention (shared): a window, or values in the key rows")
+        if n_head % n_kv_head or qkv.shape[1] < n_head * head_dim or groups.shape[1] != 3:
+            raise KernelLibraryError("attention (shared): rows or groups of another shape")
+        if (self._want(ctx.token_request, torch.int32, "token_request", 1).numel() != n
+                or self._want(ctx.positions, torch.int32, "positions", 1).numel() != n):
+            raise KernelLibraryError("attention (shared): one request and one position per row")
+        if shared.max_rows < 1 or shared.max_tokens < 0 or shared.max_behind < 1:
+            raise KernelLibraryError("attention (shared): bounds below one row or one key")
+        out = torch.empty((n, n_head * head_dim), dtype=qkv.dtype, device=self.device)
+        if n == 0:
+            return out
+        sizes = (groups.shape[0], int(shared.max_rows), int(shared.max_tokens), int(shared.max_behind))
+        floats = self.lib.mg_attention_shared_scratch_floats(*sizes, n, n_head, n_kv_head, head_dim)
+        scratch = torch.empty((floats,), dtype=torch.float32, device=self.device)
+        self._run(self.lib.mg_attention_shared(
+            _ptr(qkv), qkv.shape[1], _ptr(k), _ptr(v), _ptr(table), _ptr(ctx.token_request), _ptr(ctx.positions), _ptr(groups),
+            *sizes, _ptr(out), _ptr(scratch), n, n_head, n_kv_head, head_dim, cache.page_tokens, table.shape[1], k.shape[0],
+            table.shape[0], float(scale), is_bf16, self._stream()), "paged_attention (shared)")
+        self.launches += 1                                       # the ranges joined
         return out
 
     def head_prepare(self, proj, n_head, n_kv_head, head_dim, v_dim, q_off, k_off, v_off, unit_norm, eps,
@@ -1761,6 +1832,139 @@ class CudaOps:
         self._run(self.lib.mg_sample(_ptr(logits), _ptr(temperature), _ptr(top_k), _ptr(top_p),
                                  _ptr(seed_lo), _ptr(seed_hi), _ptr(counter), _ptr(out), rows,
                                  logits.shape[1], int(vocab_limit or 0), self._stream()), "sample")
+        return out
+
+    # ---- beam search ------------------------------------------------------------------------------
+    def beam_select(self, logits, scores, beams, ended=None, lengths=None, end_token=None, length_penalty=0.0,
+                    vocab_limit=None, out=None):
+        """The best ``beams`` continuations of every group of rows.  ``scores`` (32-bit ``[groups, in_beams]``, ``in_beams`` from 1
+        to ``beams``): the sums of the rows' log probabilities so far; ``logits`` (32-bit ``[groups * in_beams, vocab]``).  A
+        continuation of row ``b`` by id ``t`` is worth ``score_b + log_softmax(logits_b)_t`` and ranked by that over
+        ``length ** length_penalty``, its length being ``lengths[b] + 1`` (int32 per row; without a penalty they may be left
+        out).  Equal ranks go to the lower row, in a row to the larger logit and then the lower id; a logit or a value that is
+        no number counts as minus infinity.  A row that has ``ended`` (int32, not 0) has one continuation, itself, by
+        ``end_token``.  ``vocab_limit``: ids at or above it do not exist.
+
+        A beam that goes on keeps its row: its best continuation takes the row, its others take the rows whose beams do not go
+        on, by rank.  So ``parents[parents[r]] == parents[r]``, which ``beam_reorder`` relies on.  Returns a ``BeamChoice``;
+        ``out``: one of the same sizes to write into, whose tensors may be the inputs where ``in_beams == beams``."""
+        self._want(logits, torch.float32, "logits", 2)
+        groups, in_beams = self._want(scores, torch.float32, "scores", 2).shape
+        rows, vocab = logits.shape
+        limit = min(int(vocab_limit), vocab) if vocab_limit else vocab
+        if not 1 <= beams <= MAX_BEAMS or not 1 <= in_beams <= beams or rows != groups * in_beams:
+            raise KernelLibraryError(f"beam_select: {groups} groups of {in_beams} rows, {rows} rows of logits, {beams} beams (1 to {MAX_BEAMS})")
+        if limit < beams:
+            raise KernelLibraryError(f"beam_select: {beams} beams of {limit} ids")
+        for name, t in (("ended", ended), ("lengths", lengths)):
+            if t is not None and self._want(t, torch.int32, name, 1).numel() != rows:
+                raise KernelLibraryError(f"beam_select: {name} does not match the rows")
+        length_penalty = float(length_penalty)
+        if not math.isfinite(length_penalty) or (length_penalty and lengths is None):
+            raise KernelLibraryError("beam_select: a length penalty that is no number, or without lengths")
+        if end_token is None and ended is not None:
+            raise KernelLibraryError("beam_select: ended beams without an end_token")
+        if end_token is not None and not 0 <= int(end_token) < limit:
+            raise KernelLibraryError(f"beam_select: end_token {end_token} is outside the vocabulary")
+        end = -1 if end_token is None else int(end_token)
+        n = groups * beams
+        if out is None:
+            tokens, parents, ranks, over, counts, values = torch.empty((6, n), dtype=torch.int32, device=self.device).unbind(0)
+            out = BeamChoice(tokens, parents, values.view(torch.float32).view(groups, beams), ranks, over if end >= 0 else None,
+                             counts if lengths is not None else None)
+        else:
+            for name, t, wanted in (("tokens", out.tokens, True), ("parents", out.parents, True), ("ranks", out.ranks, True),
+                                    ("ended", out.ended, end >= 0), ("lengths", out.lengths, lengths is not None)):
+                if (t is not None) != wanted or (wanted and self._want(t, torch.int32, name, 1).numel() != n):
+                    raise KernelLibraryError(f"beam_select: no room for {name}")
+            if tuple(self._want(out.scores, torch.float32, "scores", 2).shape) != (groups, beams):
+                raise KernelLibraryError("beam_select: no room for scores")
+        if n == 0:
+            return out
+        scratch = torch.empty((self.lib.mg_beam_select_scratch_bytes(groups, in_beams, beams, limit),), dtype=torch.uint8,
+                              device=self.device)
+        self._run(self.lib.mg_beam_select(
+            _ptr(logits), _ptr(scores), _ptr(ended), _ptr(lengths), groups, in_beams, beams, vocab, limit, end, length_penalty,
+            _ptr(out.tokens), _ptr(out.parents), _ptr(out.scores), _ptr(out.ranks), _ptr(out.ended), _ptr(out.lengths),
+            _ptr(scratch), self._stream()), "beam_select")
+        self.launches += 1                                       # the choice
+        return out
+
+    def beam_reorder(self, parents, lengths, block_tables, k_pages, v_pages, slots=None, states=()):
+        """Hand the caches of the rows whose parent is another row over to them, in place: row ``r`` takes over, from row
+        ``parents[r]``, the block table's columns of the pages that the parent has filled (``lengths[parents[r]]`` tokens are in
+        the cache), the tokens in the parent's part-filled page (copied into the page that ``r``'s table has in that column,
+        which has to be ``r``'s own), and what the parent's slot of every state tensor holds.
+
+        Per cache group a block table (int32 ``[rows, columns]``), the keys ``[layers, pages, kv heads, page tokens, size]`` (or
+        of one layer, without the first dimension) and the values (None: they live in the keys); ``slots`` (int32 per row) and
+        ``states`` (``[slot, ...]`` each, any type).  ``parents`` as ``beam_select`` leaves them: a parent is its own parent (a row
+        whose parent is not is left alone), so nothing that is read is written."""
+        rows = self._want(parents, torch.int32, "parents", 1).numel()
+        if not len(block_tables) == len(k_pages) == len(v_pages):
+            raise KernelLibraryError("beam_reorder: one block table, keys and values per group of pages")
+        if block_tables and self._want(lengths, torch.int32, "lengths", 1).numel() != rows:
+            raise KernelLibraryError("beam_reorder: one length per row")
+        sizes = []
+        for table, k, v in zip(block_tables, k_pages, v_pages):
+            if self._want(table, torch.int32, "block_table", 2).shape[0] != rows:
+                raise KernelLibraryError("beam_reorder: one row of the block table per row")
+            self._want(k, None, "k_pages")
+            if k.dim() not in (4, 5) or (v is not None and (self._want(v, k.dtype, "v_pages").shape[:-1] != k.shape[:-1])):
+                raise KernelLibraryError("beam_reorder: keys and values of shapes that do not fit")
+            layers, (pages, heads, page_tokens, size) = (k.shape[0] if k.dim() == 5 else 1), k.shape[-4:]
+            if v is not None and v.data_ptr() == k.data_ptr():
+                v = None
+            size *= k.element_size()
+            sizes += [layers, pages, heads, page_tokens, size, v.shape[-1] * v.element_size() if v is not None else size, table.shape[1]]
+        if states and (slots is None or self._want(slots, torch.int32, "slots", 1).numel() != rows):
+            raise KernelLibraryError("beam_reorder: one state slot per row")
+        for state in states:
+            if self._want(state, None, "state").dim() < 1 or state.shape[0] == 0:
+                raise KernelLibraryError("beam_reorder: a state without slots")
+        states = [s for s in states if s.numel()]
+        if rows == 0 or not (sizes or states):
+            return
+        self._run(self.lib.mg_beam_reorder(
+            _ptr(parents), _ptr(lengths), _ptr(slots), rows, len(block_tables), _pointers(block_tables), _pointers(k_pages),
+            _pointers([None if v is not None and v.data_ptr() == k.data_ptr() else v for k, v in zip(k_pages, v_pages)]),
+            (ctypes.c_int * len(sizes))(*sizes), len(states), _pointers(states),
+            (ctypes.c_longlong * len(states))(*(s.numel() // s.shape[0] * s.element_size() for s in states)),
+            (ctypes.c_int * len(states))(*(s.shape[0] for s in states)), self._stream()), "beam_reorder")
+
+    def step_tables(self, pages, page_tokens, ctx_before, q_len, num_tokens, rows=None):
+        """A step's integers from the lengths of its requests, on the device: request ``r`` has ``ctx_before[r]`` tokens in
+        the cache and brings ``q_len[r]`` (int32 ``[R]`` each; 0: none).  ``pages``: per cache group the pages of all requests
+        there are (int32 ``[pool rows, columns]``, below zero: none), request ``r``'s in row ``rows[r]`` (int32; None: row ``r``);
+        ``page_tokens``: per group its page size.  ``num_tokens``: rows of the step; those behind the last request's tokens are
+        padding (position and cache row -1).  Returns ``StepTables``: block tables ``[R, columns]`` with -1 behind a request's
+        last page, cache rows -1 where a position has no page."""
+        R = self._want(ctx_before, torch.int32, "ctx_before", 1).numel()
+        if self._want(q_len, torch.int32, "q_len", 1).numel() != R or (
+                rows is not None and self._want(rows, torch.int32, "rows", 1).numel() != R):
+            raise KernelLibraryError("step_tables: one length, one number of tokens and one row per request")
+        groups, n = len(pages), int(num_tokens)
+        if len(page_tokens) != groups or n < 0:
+            raise KernelLibraryError("step_tables: one page size per group of pages, and no fewer than no tokens")
+        pool_rows = pages[0].shape[0] if groups else R
+        widths = []
+        for pool, size in zip(pages, page_tokens):
+            if self._want(pool, torch.int32, "pages", 2).shape[0] != pool_rows or pool.shape[1] == 0 or int(size) < 1:
+                raise KernelLibraryError("step_tables: pages or page sizes that do not fit")
+            widths.append(pool.shape[1])
+        if rows is None and R > pool_rows:
+            raise KernelLibraryError("step_tables: fewer rows of pages than requests")
+        if R == 0:
+            raise KernelLibraryError("step_tables: no requests")
+        per_token = torch.empty((2 + groups, n), dtype=torch.int32, device=self.device).unbind(0)
+        tables = [torch.empty((R, width), dtype=torch.int32, device=self.device) for width in widths]
+        out = StepTables(per_token[0], per_token[1], torch.empty((R,), dtype=torch.int32, device=self.device), tables,
+                         list(per_token[2:]))
+        ints = ctypes.c_int * groups
+        self._run(self.lib.mg_step_tables(
+            _ptr(rows), _ptr(ctx_before), _ptr(q_len), _ptr(out.token_request), _ptr(out.positions), _ptr(out.req_q_start), R, n,
+            pool_rows, groups, _pointers(pages), _pointers(tables), _pointers(out.slot_mapping), ints(*widths),
+            ints(*(int(p) for p in page_tokens)), self._stream()), "step_tables")
         return out
 
 

@@ -52,6 +52,18 @@ class StepPlan:
 
 
 @dataclass
+class SharedPrefix:
+    """Groups of a step's rows whose requests have their first tokens in common (the beams of a search, the samples of one
+    prompt): the attention may read the keys and values of those tokens once for a whole group.  It is a hint; the
+    rows' block tables lead to all their keys as ever."""
+
+    groups: torch.Tensor                  # int32 [G, 3] on the device: first row, rows, tokens they share
+    max_rows: int                         # bounds that hold for every step the context is used for (bounds that are too
+    max_tokens: int                       # low cost time): rows of a group, tokens it shares,
+    max_behind: int                       # and keys that a row sees behind them (rows of no group: all they see)
+
+
+@dataclass
 class StepContext:
     ops: Any                              # the kernel set the parts call
     act_dtype: torch.dtype                # compute dtype between norm and projection
@@ -90,6 +102,8 @@ class StepContext:
     max_ctx_after: int = 0                # longest context once this step's tokens are in
     decode_only: bool = False             # every request brings exactly one token
     storage: Any = None                   # cache.storage.CacheStorage
+    # Optional: rows that have their first tokens in common (steps of single tokens only)
+    shared_prefix: SharedPrefix | None = None
 
     def cache_view(self, cache_layer: int, writes: bool = True):
         return self.storage.layer_view(cache_layer, writes) if self.storage is not None else None
