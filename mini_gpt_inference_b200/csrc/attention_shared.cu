@@ -62,6 +62,69 @@ __device__ __forceinline__ int group_tokens(const SharedArgs& a, int row, int* h
     return *hold;
 }
 
+// What a CTA works on: (row, head) pairs of `rows` rows and the keys key0 .. key1 - 1 that their ranges `slot` hold.
+struct Item {
+    int first_row, rows, tile, tiles, key0, key1, slot, shared_keys;
+    bool shared;
+    const int* table;
+};
+
+// False if there is nothing to do.  All threads of the CTA call it.
+__device__ __forceinline__ bool item_of(const SharedArgs& a, int item, int* hold, Item& it) {
+    const int shared_items = a.n_groups * a.row_tiles * a.shared_slots;
+    it.shared = item < shared_items;
+    it.shared_keys = 0;
+    it.tile = 0;
+    it.tiles = it.rows = 1;
+    if (it.shared) {
+        it.slot = item % a.shared_slots;
+        item /= a.shared_slots;
+        it.tile = item % a.row_tiles;
+        it.tiles = a.row_tiles;
+        const int g = item / a.row_tiles;
+        it.first_row = a.groups[3 * g];
+        it.rows = a.groups[3 * g + 1];
+        it.shared_keys = a.groups[3 * g + 2];
+        if (it.first_row < 0 || it.rows <= 0 || it.first_row >= a.n) return false;
+        it.rows = min(it.rows, a.n - it.first_row);
+        const int step = range_keys(it.shared_keys, a.shared_slots, SHARED_LEAST);
+        it.key0 = it.slot * step;
+        it.key1 = min(it.shared_keys, it.key0 + step);
+    } else {
+        item -= shared_items;
+        it.slot = item % a.own_slots;
+        it.first_row = item / a.own_slots;
+        const int p = a.positions[it.first_row];
+        int behind = group_tokens(a, it.first_row, hold);
+        if (behind > p + 1) behind = 0;
+        const int step = range_keys(p + 1 - behind, a.own_slots, OWN_LEAST);
+        it.key0 = behind + it.slot * step;
+        it.key1 = min(p + 1, it.key0 + step);
+        it.slot += a.shared_slots;
+    }
+    int request = a.token_request[it.first_row];
+    if (!MG_GUARDED(attention_shared, MG_GUARD_REQUEST, request, a.n_requests)) request = 0;
+    it.table = a.table + (size_t)request * a.max_pages;
+    return it.key0 < it.key1;
+}
+
+// Row of the pool, seen as [page * kv head * token][D], of the key at a position; -1: it has no page (and is not there).
+__device__ __forceinline__ int cache_row(const SharedArgs& a, const Item& it, int position, int kv_head) {
+    if (position >= it.key1) return -1;
+    const int pi = position / a.page_tokens;
+    int page = pi < a.max_pages ? it.table[pi] : -1;
+    if (page >= 0 && !MG_GUARDED(attention_shared, MG_GUARD_PAGE, page, a.num_pages)) page = -1;
+    if (page < 0 || page >= a.num_pages) return -1;
+    return (page * a.n_kv_head + kv_head) * a.page_tokens + position - pi * a.page_tokens;
+}
+
+// The row of pair j of an item, or -1: pairs behind the last one, and rows that do not see all the shared keys.
+__device__ __forceinline__ int pair_row(const SharedArgs& a, const Item& it, int j, int share) {
+    if (j >= it.rows * share) return -1;
+    const int row = it.first_row + j / share;
+    return !it.shared || a.positions[row] + 1 >= it.shared_keys ? row : -1;
+}
+
 // ---- any head size, either type: 16 (row, head) pairs and 64 keys at a time, in 32-bit arithmetic ------------------------
 constexpr int SIMT_THREADS = 128, SIMT_QUERIES = 16;
 
@@ -78,52 +141,13 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_shared_simt_kernel(Sha
     float* p_s = k_s + BLOCK_KEYS * (D + 1);             // [64][16]
     const int lanes = simt_lanes(D), dl = tid % lanes, ks = tid / lanes, key_parts = SIMT_THREADS / lanes;
 
-    // which queries and which keys
-    const int shared_items = a.n_groups * a.row_tiles * a.shared_slots;
-    int item = blockIdx.x, first_row, rows, key0, key1, slot, tile, tiles;
-    const bool shared = item < shared_items;
-    if (shared) {
-        slot = item % a.shared_slots;
-        item /= a.shared_slots;
-        tile = item % a.row_tiles;
-        tiles = a.row_tiles;
-        const int g = item / a.row_tiles;
-        first_row = a.groups[3 * g];
-        rows = a.groups[3 * g + 1];
-        const int keys = a.groups[3 * g + 2], step = range_keys(keys, a.shared_slots, SHARED_LEAST);
-        key0 = slot * step;
-        key1 = min(keys, key0 + step);
-        if (first_row < 0 || rows <= 0 || first_row >= a.n) return;
-        rows = min(rows, a.n - first_row);
-    } else {
-        item -= shared_items;
-        slot = item % a.own_slots;
-        first_row = item / a.own_slots;
-        rows = 1;
-        tile = 0;
-        tiles = 1;
-        const int p = a.positions[first_row];
-        int behind = group_tokens(a, first_row, &hold);
-        if (behind > p + 1) behind = 0;
-        const int step = range_keys(p + 1 - behind, a.own_slots, OWN_LEAST);
-        key0 = behind + slot * step;
-        key1 = min(p + 1, key0 + step);
-        slot += a.shared_slots;
-    }
-    if (key0 >= key1) return;
-    int request = a.token_request[first_row];
-    if (!MG_GUARDED(attention_shared, MG_GUARD_REQUEST, request, a.n_requests)) request = 0;
-    const int* table = a.table + (size_t)request * a.max_pages;
-    const int shared_keys = shared ? a.groups[3 * (blockIdx.x / (a.shared_slots * a.row_tiles)) + 2] : 0;
-
-    for (int q0 = tile * SIMT_QUERIES; q0 < rows * share; q0 += tiles * SIMT_QUERIES) {
+    Item it;
+    if (!item_of(a, blockIdx.x, &hold, it)) return;
+    for (int q0 = it.tile * SIMT_QUERIES; q0 < it.rows * share; q0 += it.tiles * SIMT_QUERIES) {
         __syncthreads();
         if (tid < SIMT_QUERIES) {
-            const int j = q0 + tid, row = first_row + j / share;
-            // (a row that does not see all the shared keys is no row of this range)
-            const bool in = j < rows * share && (!shared || a.positions[row] + 1 >= shared_keys);
-            q_token[tid] = in ? row : -1;
-            q_head[tid] = kv_head * share + j % share;
+            q_token[tid] = pair_row(a, it, q0 + tid, share);
+            q_head[tid] = kv_head * share + (q0 + tid) % share;
             q_max[tid] = -INFINITY;
             q_sum[tid] = 0.f;
         }
@@ -138,16 +162,9 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_shared_simt_kernel(Sha
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int j = 0; j < SIMT_QUERIES; ++j) acc[i][j] = 0.f;
-        for (int b0 = key0; b0 < key1; b0 += BLOCK_KEYS) {
+        for (int b0 = it.key0; b0 < it.key1; b0 += BLOCK_KEYS) {
             __syncthreads();
-            if (tid < BLOCK_KEYS) {
-                const int pos = b0 + tid, pi = pos / a.page_tokens;
-                int page = pos < key1 && pi < a.max_pages ? table[pi] : -1;
-                if (page >= 0 && !MG_GUARDED(attention_shared, MG_GUARD_PAGE, page, a.num_pages)) page = -1;
-                if (page >= a.num_pages) page = -1;      // a key without a page is not there
-                krow[tid] = page < 0 ? -1 : pos - pi * a.page_tokens;
-                if (page >= 0) krow[tid] += (page * a.n_kv_head + kv_head) * a.page_tokens;
-            }
+            if (tid < BLOCK_KEYS) krow[tid] = cache_row(a, it, b0 + tid, kv_head);
             __syncthreads();
             for (int i = tid; i < BLOCK_KEYS * D; i += SIMT_THREADS) {
                 const int r = i / D, d = i - r * D;
@@ -225,12 +242,261 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_shared_simt_kernel(Sha
 #pragma unroll
             for (int j = 0; j < SIMT_QUERIES; ++j) {
                 if (q_token[j] < 0) continue;
-                const size_t at = ((size_t)q_token[j] * a.n_head + q_head[j]) * slots + slot;
+                const size_t at = ((size_t)q_token[j] * a.n_head + q_head[j]) * slots + it.slot;
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
                     if (dl + i * SIMT_THREADS < D) a.part_out[at * D + dl + i * SIMT_THREADS] = acc[i][j];
                 if (dl == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(q_max[j], q_sum[j]);
             }
+    }
+}
+
+// ---- bfloat16, heads of a multiple of 8 features: the warp-level tensor cores ------------------------------------------
+// Keys are the rows of the products, pairs their columns (S = K q^T, 16 keys x 8 pairs; O = V^T P, 16 features x 8 pairs), so
+// that a row's own keys, read for one pair or a few, waste little.  A CTA's four warps take 16 keys in turn; each copies its
+// own rows from their pages (cp.async, a ring of stages), and keeps maximum, sum and average of its own, so the loop has no
+// barrier.  The maximum is a reference that moves only when a score is more than 2^REF_SLACK above it: then everything so
+// far is rescaled.  P goes into the product rounded to bfloat16 (2^-8 of a weight at most, as in the other attention
+// kernels of this type), the sums are of the 32-bit weights.
+constexpr float REF_SLACK = 8.f;
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Transpose of an 8x8 block of 16-bit values held one row per group of four lanes.
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+constexpr int MMA_THREADS = 128, MMA_WARPS = MMA_THREADS / 32, UNIT = 16;       // keys a warp takes at a time
+
+// Sizes by padded head: DP features (32, 64, 128 or 256), of which D are there and the others zero.
+template <int DP>
+struct MmaSizes {
+    static constexpr int STAGES = DP <= 64 ? 4 : DP == 128 ? 3 : 2;
+    static constexpr int TILE = UNIT * DP * 2;                          // bytes of 16 keys or values
+    static constexpr size_t SMEM = (size_t)MMA_WARPS * STAGES * 2 * TILE;
+};
+
+template <int DP, int NT>      // NT: tiles of 8 pairs that a CTA takes at once
+__global__ void __launch_bounds__(MMA_THREADS) attention_shared_mma_kernel(SharedArgs a) {
+    using Z = MmaSizes<DP>;
+    constexpr int STAGES = Z::STAGES, CPR = DP / 8, ROWB = 2 * DP;
+    constexpr int RPL = CPR >= 8 ? 1 : 8 / CPR, SWZ = CPR >= 8 ? 8 : CPR;     // piece c of row r lies at piece c ^ ((r / RPL) % SWZ)
+    constexpr int PSTRIDE = DP + 2;                                     // floats of a warp's partial: O, maximum, sum
+    static_assert((size_t)MMA_WARPS * NT * 8 * PSTRIDE * 4 <= Z::SMEM, "the warps' results meet where the tiles were");
+    extern __shared__ __align__(128) uint8_t ring[];
+    __shared__ int hold;
+    __shared__ uint32_t valid[MMA_WARPS][STAGES];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int kv_head = blockIdx.y, share = a.n_head / a.n_kv_head, D = a.D, pieces = D / 8;
+    const bf16* const k_pages = (const bf16*)a.k_pages;
+    const bf16* const v_pages = (const bf16*)a.v_pages;
+    Item it;
+    if (!item_of(a, blockIdx.x, &hold, it)) return;
+    uint8_t* const mine = ring + (size_t)warp * STAGES * 2 * Z::TILE;
+    const uint32_t mine_u = (uint32_t)__cvta_generic_to_shared(mine);
+    const uint4 zero4 = make_uint4(0u, 0u, 0u, 0u);
+    const int units = (it.key1 - it.key0 + UNIT - 1) / UNIT, my_units = units > warp ? (units - warp + MMA_WARPS - 1) / MMA_WARPS : 0;
+
+    for (int q0 = it.tile * NT * 8; q0 < it.rows * share; q0 += it.tiles * NT * 8) {
+        const int nts = min(NT, (it.rows * share - q0 + 7) / 8);       // tiles of pairs that there are
+        if (pieces < CPR) {                                             // features that are not there: zeros in every stage
+            for (int i = lane; i < STAGES * 2 * UNIT * (CPR - pieces); i += 32) {
+                const int r = i / (CPR - pieces), c = pieces + i % (CPR - pieces);
+                *reinterpret_cast<uint4*>(mine + r * ROWB + ((c ^ (((r % UNIT) / RPL) % SWZ)) * 16)) = zero4;
+            }
+        }
+        // the first units' rows of the pool, then the copies; the row of the unit after the last one asked for is on its way
+        auto row_of = [&](int n) {                                      // lane i: row of key i of this warp's n-th unit
+            return n < my_units ? cache_row(a, it, it.key0 + (warp + n * MMA_WARPS) * UNIT + (lane & 15), kv_head) : -1;
+        };
+        auto load = [&](int n, int row) {
+            if (n < my_units) {
+                const uint32_t there = __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
+                if (lane == 0) valid[warp][n % STAGES] = there;
+                const uint32_t at = (uint32_t)(n % STAGES) * 2 * Z::TILE;
+#pragma unroll
+                for (int i0 = 0; i0 < UNIT * CPR; i0 += 32) {
+                    const int i = i0 + lane, r = i / CPR, c = i % CPR;
+                    const int from = __shfl_sync(0xffffffffu, row, r);
+                    const uint32_t off = at + r * ROWB + ((c ^ ((r / RPL) % SWZ)) * 16);
+                    if (c < pieces) {
+                        if (from >= 0) {
+                            cp_async16(mine_u + off, k_pages + (size_t)from * D + c * 8);
+                            cp_async16(mine_u + off + Z::TILE, v_pages + (size_t)from * D + c * 8);
+                        } else {                                        // keeps 0 * garbage out of the product
+                            *reinterpret_cast<uint4*>(mine + off) = zero4;
+                            *reinterpret_cast<uint4*>(mine + off + Z::TILE) = zero4;
+                        }
+                    }
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        int row = row_of(0);
+#pragma unroll
+        for (int n = 0; n < STAGES - 1; ++n) {
+            const int next = row_of(n + 1);
+            load(n, row);
+            row = next;
+        }
+        // the pairs' queries as the B operand: pair nt * 8 + g in column g
+        uint32_t qb[NT][DP / 16][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int j = q0 + nt * 8 + g, token = nt < nts ? pair_row(a, it, j, share) : -1;
+            const bf16* const q = (const bf16*)a.q + (token < 0 ? 0 : token * a.q_stride + (size_t)(kv_head * share + j % share) * D);
+#pragma unroll
+            for (int ks = 0; ks < DP / 16; ++ks)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int d = ks * 16 + h * 8 + 2 * t;
+                    qb[nt][ks][h] = token >= 0 && d < D ? *reinterpret_cast<const uint32_t*>(q + d) : 0u;
+                }
+        }
+        float o[NT][DP / 16][4], ref[NT][2], sum[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            ref[nt][0] = ref[nt][1] = -INFINITY;
+            sum[nt][0] = sum[nt][1] = 0.f;
+#pragma unroll
+            for (int dm = 0; dm < DP / 16; ++dm)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[nt][dm][i] = 0.f;
+        }
+        // ldmatrix addresses: K as the A operand (matrix j = lane / 8: keys (j % 2) * 8 .., piece j / 2), V transposed (keys
+        // (j / 2) * 8 .., piece j % 2)
+        const int krow = (lane & 7) + (((lane >> 3) & 1) << 3), kpiece = lane >> 4;
+        const int vrow = (lane & 7) + (((lane >> 4) & 1) << 3), vpiece = (lane >> 3) & 1;
+        for (int n = 0; n < my_units; ++n) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+            __syncwarp();                                               // this unit has landed, the one before is used up
+            const int next = row_of(n + STAGES);
+            load(n + STAGES - 1, row);
+            row = next;
+            const uint32_t k_at = mine_u + (uint32_t)(n % STAGES) * 2 * Z::TILE, v_at = k_at + Z::TILE;
+            const uint32_t there = valid[warp][n % STAGES];
+            float s[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < DP / 16; ++ks) {
+                uint32_t f[4];
+                ldmatrix_x4(f, k_at + krow * ROWB + (((ks * 2 + kpiece) ^ ((krow / RPL) % SWZ)) * 16));
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                    if (nt < nts) mma_bf16(s[nt], f, qb[nt][ks][0], qb[nt][ks][1]);
+            }
+            // a lane holds pairs 2t, 2t+1 (numbers 0, 1 and 2, 3) of keys g and g + 8
+            bool above = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[nt][i] = (there >> (g + ((i >> 1) << 3))) & 1u ? s[nt][i] * a.scale_log2e : -INFINITY;
+                    above = above || (nt < nts && !(s[nt][i] <= ref[nt][i & 1] + REF_SLACK));
+                }
+            if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float top = fmaxf(ref[nt][i], fmaxf(s[nt][i], s[nt][i + 2]));
+#pragma unroll
+                        for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                        const float corr = ref[nt][i] == -INFINITY ? 0.f : exp2f(ref[nt][i] - top);
+                        ref[nt][i] = top;
+                        sum[nt][i] *= corr;
+#pragma unroll
+                        for (int dm = 0; dm < DP / 16; ++dm) {
+                            o[nt][dm][i] *= corr;
+                            o[nt][dm][i + 2] *= corr;
+                        }
+                    }
+            }
+            uint32_t pb[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float e[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    e[i] = exp2_approx(s[nt][i] - (ref[nt][i & 1] == -INFINITY ? 0.f : ref[nt][i & 1]));
+                    sum[nt][i & 1] += e[i];
+                }
+                pb[nt][0] = movmatrix_trans(pack_bf16(e[0], e[1]));
+                pb[nt][1] = movmatrix_trans(pack_bf16(e[2], e[3]));
+            }
+#pragma unroll
+            for (int dm = 0; dm < DP / 16; ++dm) {
+                uint32_t f[4];
+                ldmatrix_x4_trans(f, v_at + vrow * ROWB + (((dm * 2 + vpiece) ^ ((vrow / RPL) % SWZ)) * 16));
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                    if (nt < nts) mma_bf16(o[nt][dm], f, pb[nt][0], pb[nt][1]);
+            }
+        }
+        // the warps' results meet in shared memory
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();
+        float* const part = reinterpret_cast<float*>(ring);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) sum[nt][i] += __shfl_xor_sync(0xffffffffu, sum[nt][i], x);
+                float* const dst = part + (warp * NT * 8 + nt * 8 + 2 * t + i) * PSTRIDE;
+#pragma unroll
+                for (int dm = 0; dm < DP / 16; ++dm) {
+                    dst[dm * 16 + g] = o[nt][dm][i];
+                    dst[dm * 16 + g + 8] = o[nt][dm][i + 2];
+                }
+                if (g == 0) {
+                    dst[DP] = ref[nt][i];
+                    dst[DP + 1] = sum[nt][i];
+                }
+            }
+        __syncthreads();
+        const int slots = a.shared_slots + a.own_slots;
+        for (int e = tid; e < nts * 8 * DP; e += MMA_THREADS) {
+            const int j = e / DP, d = e % DP, token = pair_row(a, it, q0 + j, share);
+            if (token < 0 || d >= D) continue;
+            float top = -INFINITY, v = 0.f, l = 0.f;
+#pragma unroll
+            for (int w = 0; w < MMA_WARPS; ++w) top = fmaxf(top, part[(w * NT * 8 + j) * PSTRIDE + DP]);
+#pragma unroll
+            for (int w = 0; w < MMA_WARPS; ++w) {                       // warps in order
+                const float* const src = part + (w * NT * 8 + j) * PSTRIDE;
+                const float f = src[DP] == -INFINITY ? 0.f : exp2f(src[DP] - top);
+                v = fmaf(f, src[d], v);
+                l = fmaf(f, src[DP + 1], l);
+            }
+            const size_t at = ((size_t)token * a.n_head + kv_head * share + (q0 + j) % share) * slots + it.slot;
+            a.part_out[at * D + d] = v;
+            if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(top, l);
+        }
+        __syncthreads();                                                // (the tiles are loaded again for the next pairs)
     }
 }
 
@@ -275,39 +541,66 @@ __global__ void __launch_bounds__(128) attention_shared_join_kernel(SharedArgs a
 }
 
 template <typename T>
-int launch_simt(const SharedArgs& a, cudaStream_t s) {
-    const size_t smem = sizeof(float) * ((size_t)a.D * SIMT_QUERIES + (size_t)BLOCK_KEYS * (a.D + 1) + BLOCK_KEYS * SIMT_QUERIES);
-    const cudaError_t e = mg_raise_shared(attention_shared_simt_kernel<T>, smem);
-    if (e != cudaSuccess) return mg_set_error(MG_ERR_CUDA, "attention (shared): cannot raise shared memory: %s", cudaGetErrorString(e));
-    const long long items = (long long)a.n_groups * a.row_tiles * a.shared_slots + (long long)a.n * a.own_slots;
-    attention_shared_simt_kernel<T><<<dim3((unsigned)items, a.n_kv_head), SIMT_THREADS, smem, s>>>(a);
-    MG_CHECK_LAUNCH("attention (shared)");
+int launch_join(const SharedArgs& a, cudaStream_t s) {
     attention_shared_join_kernel<T><<<dim3(a.n, ceil_div(a.n_head, 4)), 128, 0, s>>>(a);
     MG_CHECK_LAUNCH("attention (shared, join)");
     return MG_OK;
 }
 
-// How a launch is cut: [0] CTAs that share the pairs of a group, [1] ranges of shared keys, [2] ranges of own keys.
-void cut(int n_groups, int max_rows, int max_tokens, int max_behind, int n, int n_head, int n_kv_head, int* out) {
-    const int share = n_head / n_kv_head;
-    out[0] = ceil_div(max_rows * share, SIMT_QUERIES);
-    const long long shared_ctas = (long long)n_groups * out[0] * n_kv_head, own_ctas = (long long)n * n_kv_head;
+template <typename... KArgs>
+int launch_ranges(void (*kernel)(KArgs...), int threads, size_t smem, const SharedArgs& a, cudaStream_t s) {
+    const cudaError_t e = mg_raise_shared(kernel, smem);
+    if (e != cudaSuccess) return mg_set_error(MG_ERR_CUDA, "attention (shared): cannot raise shared memory: %s", cudaGetErrorString(e));
+    const long long items = (long long)a.n_groups * a.row_tiles * a.shared_slots + (long long)a.n * a.own_slots;
+    kernel<<<dim3((unsigned)items, a.n_kv_head), threads, smem, s>>>(a);
+    MG_CHECK_LAUNCH("attention (shared)");
+    return MG_OK;
+}
+
+template <int DP>
+int launch_mma(const SharedArgs& a, int pair_tiles, cudaStream_t s) {
+    constexpr size_t smem = MmaSizes<DP>::SMEM;
+    if (pair_tiles == 1) return launch_ranges(attention_shared_mma_kernel<DP, 1>, MMA_THREADS, smem, a, s);
+    if constexpr (DP <= 128)
+        if (pair_tiles == 2) return launch_ranges(attention_shared_mma_kernel<DP, 2>, MMA_THREADS, smem, a, s);
+    if constexpr (DP <= 64)
+        if (pair_tiles == 4) return launch_ranges(attention_shared_mma_kernel<DP, 4>, MMA_THREADS, smem, a, s);
+    return mg_set_error(MG_ERR_ARG, "attention (shared): no kernel for %d tiles of pairs", pair_tiles);
+}
+
+int padded_head(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+
+// How a launch is cut.
+struct Cut {
+    bool mma;            // the warp-level tensor cores, or 32-bit arithmetic
+    int pair_tiles;      // mma: tiles of 8 pairs that a CTA takes at once
+    int row_tiles;       // CTAs that share the pairs of a group
+    int shared_slots, own_slots;      // ranges of shared keys, and of a row's own
+};
+Cut cut(int n_groups, int max_rows, int max_tokens, int max_behind, int n, int n_head, int n_kv_head, int head_dim, bool is_bf16) {
+    Cut c;
+    const int share = n_head / n_kv_head, pairs = n_groups > 0 ? (max_rows < n ? max_rows : n) * share : share;
+    c.mma = is_bf16 && head_dim % 8 == 0;
+    const int most_tiles = head_dim <= 64 ? 4 : head_dim <= 128 ? 2 : 1;      // what the registers hold
+    c.pair_tiles = pairs <= 8 ? 1 : pairs <= 16 && most_tiles > 1 ? 2 : most_tiles;
+    c.row_tiles = ceil_div(pairs, c.mma ? 8 * c.pair_tiles : SIMT_QUERIES);
+    const long long shared_ctas = (long long)n_groups * c.row_tiles * n_kv_head, own_ctas = (long long)n * n_kv_head;
     const int most_shared = ceil_div(max_tokens > 0 ? max_tokens : 1, SHARED_LEAST), most_own = ceil_div(max_behind, OWN_LEAST);
     const long long want = 148 * 4;
-    long long a = shared_ctas > 0 ? (want + shared_ctas - 1) / shared_ctas : 1, b = (want + own_ctas - 1) / own_ctas;
-    out[1] = (int)(a < 1 ? 1 : a > most_shared ? most_shared : a);
-    out[2] = (int)(b < 1 ? 1 : b > most_own ? most_own : b);
+    const long long x = shared_ctas > 0 ? (want + shared_ctas - 1) / shared_ctas : 1, y = (want + own_ctas - 1) / own_ctas;
+    c.shared_slots = (int)(x < 1 ? 1 : x > most_shared ? most_shared : x);
+    c.own_slots = (int)(y < 1 ? 1 : y > most_own ? most_own : y);
+    return c;
 }
 
 }  // namespace
 
 // Floats of scratch that mg_attention_shared() takes for these sizes and bounds.
 MG_API long long mg_attention_shared_scratch_floats(int n_groups, int max_rows, int max_tokens, int max_behind, int n, int n_head,
-                                                    int n_kv_head, int head_dim) {
+                                                    int n_kv_head, int head_dim, int is_bf16) {
     if (n_groups < 0 || max_rows <= 0 || n <= 0 || n_head <= 0 || n_kv_head <= 0 || n_head % n_kv_head != 0 || max_behind <= 0) return 0;
-    int c[3];
-    cut(n_groups, max_rows, max_tokens, max_behind, n, n_head, n_kv_head, c);
-    return (long long)n * n_head * (c[1] + c[2]) * (head_dim + 2);
+    const Cut c = cut(n_groups, max_rows, max_tokens, max_behind, n, n_head, n_kv_head, head_dim, is_bf16 != 0);
+    return (long long)n * n_head * (c.shared_slots + c.own_slots) * (head_dim + 2);
 }
 
 // Attention of n single query tokens, groups of which share their first keys.  q: rows of q_stride elements whose first
@@ -334,18 +627,34 @@ MG_API int mg_attention_shared(const void* q, long long q_stride, const void* k_
     if (head_dim > 256 || n_kv_head > 65535)
         return mg_set_error(MG_ERR_UNSUPPORTED, "attention (shared): head_dim %d is more than 256", head_dim);
     SharedArgs a;
-    int c[3];
-    cut(n_groups, max_rows, max_tokens, max_behind, n, n_head, n_kv_head, c);
+    const Cut c = cut(n_groups, max_rows, max_tokens, max_behind, n, n_head, n_kv_head, head_dim, is_bf16 != 0);
     a.q = q; a.q_stride = q_stride; a.k_pages = k_pages; a.v_pages = v_pages; a.table = table; a.token_request = token_request;
     a.positions = positions; a.groups = groups; a.out = out;
     a.n_groups = n_groups; a.n = n; a.n_head = n_head; a.n_kv_head = n_kv_head; a.D = head_dim; a.page_tokens = page_tokens;
     a.max_pages = max_pages; a.num_pages = num_pages; a.n_requests = n_requests;
-    a.row_tiles = c[0]; a.shared_slots = c[1]; a.own_slots = c[2];
+    a.row_tiles = c.row_tiles; a.shared_slots = c.shared_slots; a.own_slots = c.own_slots;
     a.scale_log2e = scale * 1.4426950408889634f;
-    const size_t slots = (size_t)n * n_head * (c[1] + c[2]);
+    const size_t slots = (size_t)n * n_head * (c.shared_slots + c.own_slots);
     a.part_ml = scratch;
     a.part_out = scratch + 2 * slots;
-    const long long items = (long long)n_groups * c[0] * c[1] + (long long)n * c[2];
+    const long long items = (long long)n_groups * c.row_tiles * c.shared_slots + (long long)n * c.own_slots;
     MG_REQUIRE(items < (1ll << 31), "attention (shared): too many rows");
-    return is_bf16 ? launch_simt<bf16>(a, (cudaStream_t)stream) : launch_simt<float>(a, (cudaStream_t)stream);
+    cudaStream_t s = (cudaStream_t)stream;
+    int rc;
+    if (c.mma && ((((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages) & 15) || q_stride % 2))
+        return mg_set_error(MG_ERR_ARG, "attention (shared): queries and pages have to be 16-byte aligned, rows of queries 4-byte aligned");
+    if (c.mma) {
+        switch (padded_head(head_dim)) {
+            case 32: rc = launch_mma<32>(a, c.pair_tiles, s); break;
+            case 64: rc = launch_mma<64>(a, c.pair_tiles, s); break;
+            case 128: rc = launch_mma<128>(a, c.pair_tiles, s); break;
+            default: rc = launch_mma<256>(a, c.pair_tiles, s);
+        }
+    } else {
+        const size_t smem = sizeof(float) * ((size_t)head_dim * SIMT_QUERIES + (size_t)BLOCK_KEYS * (head_dim + 1) + BLOCK_KEYS * SIMT_QUERIES);
+        rc = is_bf16 ? launch_ranges(attention_shared_simt_kernel<bf16>, SIMT_THREADS, smem, a, s)
+                     : launch_ranges(attention_shared_simt_kernel<float>, SIMT_THREADS, smem, a, s);
+    }
+    if (rc != MG_OK) return rc;
+    return is_bf16 ? launch_join<bf16>(a, s) : launch_join<float>(a, s);
 }

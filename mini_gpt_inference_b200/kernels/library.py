@@ -173,7 +173,7 @@ def load(verbose: bool = True):
     lib.mg_attention_mma_scratch_floats.restype = ctypes.c_longlong
     lib.mg_attention_split_scratch_floats.argtypes = [c_int, c_int, c_int, c_int]
     lib.mg_attention_split_scratch_floats.restype = ctypes.c_longlong
-    lib.mg_attention_shared_scratch_floats.argtypes = [c_int] * 8
+    lib.mg_attention_shared_scratch_floats.argtypes = [c_int] * 9
     lib.mg_attention_shared_scratch_floats.restype = ctypes.c_longlong
     lib.mg_beam_select_scratch_bytes.argtypes = [c_int] * 4
     lib.mg_beam_select_scratch_bytes.restype = ctypes.c_longlong

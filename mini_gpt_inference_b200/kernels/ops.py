@@ -988,7 +988,7 @@ class CudaOps:
         if n == 0:
             return out
         sizes = (groups.shape[0], int(shared.max_rows), int(shared.max_tokens), int(shared.max_behind))
-        floats = self.lib.mg_attention_shared_scratch_floats(*sizes, n, n_head, n_kv_head, head_dim)
+        floats = self.lib.mg_attention_shared_scratch_floats(*sizes, n, n_head, n_kv_head, head_dim, is_bf16)
         scratch = torch.empty((floats,), dtype=torch.float32, device=self.device)
         self._run(self.lib.mg_attention_shared(
             _ptr(qkv), qkv.shape[1], _ptr(k), _ptr(v), _ptr(table), _ptr(ctx.token_request), _ptr(ctx.positions), _ptr(groups),
