@@ -15,13 +15,14 @@
 // keys for itself, and so does one that belongs to no group.
 #include <math.h>
 
-#include "common.cuh"
+#include "blackwell.cuh"
+#include "tensor_map.cuh"
 
 MG_GUARD_DECLARE(attention_shared)
 
 namespace {
 
-constexpr int BLOCK_KEYS = 64;         // ranges are cut at multiples of this many keys
+constexpr int BLOCK_KEYS = 64;         // keys of a block of the 32-bit kernel; ranges are cut at multiples of it (shared ones: see range_keys)
 
 struct SharedArgs {
     const void* q;                     // rows whose first n_head * D columns are the queries
@@ -38,17 +39,18 @@ struct SharedArgs {
     int n_groups, n, n_head, n_kv_head, D, page_tokens, max_pages, num_pages, n_requests;
     int row_tiles;                     // CTAs that share the (row, head) pairs of a group
     int shared_slots, own_slots;       // ranges of the shared keys, and of a row's own
+    int shared_least;                  // keys of a range of shared keys, at least, and what they are a multiple of
+    int first_item;                    // item of the grid's first CTA
     float scale_log2e;
 };
 
-// Keys of one range when `keys` of them are cut into at most `slots`, each of at least `least` keys.
-__host__ __device__ __forceinline__ int range_keys(int keys, int slots, int least) {
+// Keys of one range when `keys` of them are cut into at most `slots`, each a multiple of `least` keys.
+__device__ __forceinline__ int range_keys(int keys, int slots, int least) {
     const int even = (keys + slots - 1) / slots;
-    const int whole = (even + BLOCK_KEYS - 1) / BLOCK_KEYS * BLOCK_KEYS;
-    return whole < least ? least : whole;
+    return max(1, (even + least - 1) / least) * least;
 }
 
-constexpr int SHARED_LEAST = 64, OWN_LEAST = 64;
+constexpr int OWN_LEAST = 64;
 
 // The shared tokens of the group that `row` belongs to (0: none), by all threads of a CTA; `hold` is a word of shared memory.
 __device__ __forceinline__ int group_tokens(const SharedArgs& a, int row, int* hold) {
@@ -87,7 +89,7 @@ __device__ __forceinline__ bool item_of(const SharedArgs& a, int item, int* hold
         it.shared_keys = a.groups[3 * g + 2];
         if (it.first_row < 0 || it.rows <= 0 || it.first_row >= a.n) return false;
         it.rows = min(it.rows, a.n - it.first_row);
-        const int step = range_keys(it.shared_keys, a.shared_slots, SHARED_LEAST);
+        const int step = range_keys(it.shared_keys, a.shared_slots, a.shared_least);
         it.key0 = it.slot * step;
         it.key1 = min(it.shared_keys, it.key0 + step);
     } else {
@@ -142,7 +144,7 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_shared_simt_kernel(Sha
     const int lanes = simt_lanes(D), dl = tid % lanes, ks = tid / lanes, key_parts = SIMT_THREADS / lanes;
 
     Item it;
-    if (!item_of(a, blockIdx.x, &hold, it)) return;
+    if (!item_of(a, a.first_item + blockIdx.x, &hold, it)) return;
     for (int q0 = it.tile * SIMT_QUERIES; q0 < it.rows * share; q0 += it.tiles * SIMT_QUERIES) {
         __syncthreads();
         if (tid < SIMT_QUERIES) {
@@ -313,7 +315,7 @@ __global__ void __launch_bounds__(MMA_THREADS) attention_shared_mma_kernel(Share
     const bf16* const k_pages = (const bf16*)a.k_pages;
     const bf16* const v_pages = (const bf16*)a.v_pages;
     Item it;
-    if (!item_of(a, blockIdx.x, &hold, it)) return;
+    if (!item_of(a, a.first_item + blockIdx.x, &hold, it)) return;
     uint8_t* const mine = ring + (size_t)warp * STAGES * 2 * Z::TILE;
     const uint32_t mine_u = (uint32_t)__cvta_generic_to_shared(mine);
     const uint4 zero4 = make_uint4(0u, 0u, 0u, 0u);
@@ -500,6 +502,309 @@ __global__ void __launch_bounds__(MMA_THREADS) attention_shared_mma_kernel(Share
     }
 }
 
+// ---- bfloat16, heads of 64 or 128, many pairs: the 5th-generation tensor cores --------------------------------------------
+// A CTA takes two tiles of 128 pairs and walks over the keys of its range in blocks of 128, which both tiles multiply with:
+//
+//   load warp       TMA tiles of keys and values from the pages (one copy per page, tensor and 64 features, 128-byte swizzle)
+//                   into a ring of two stages or more
+//   issue warp      S = Q K^T (128 x 128, TMEM), and O += P V (128 x head, TMEM) with P read from TMEM, where it lies in S's
+//                   place.  The tiles take turns: while one's scores are in the softmax, the other's are computed.
+//   softmax warps   four a tile, a thread a pair: its row of S into registers, 2^(s - ref) as bfloat16 back, the 32-bit sum kept.
+//                   `ref` is the first block's maximum and moves only when a score is more than 2^TC_SLACK above it: O is then
+//                   rescaled in TMEM.  (O / sum does not depend on ref; 2^TC_SLACK keeps the numbers in range.)
+//
+// What bounds it: at heads of 128 a block of 128 keys is 2 x 128 x 128 x 128 multiply-adds per product and tile, 1,024 cycles
+// of the tensor core for both, and 16,384 exponentials, 1,024 cycles of the special-function units.  All waits are bounded:
+// when one runs out, `status` gets a code, the CTA writes nothing more, frees its TMEM and returns.
+constexpr int TC_KEYS = 128, TC_PAIRS = 128, TC_TILES = 2;
+constexpr int TC_SOFTMAX_WARPS = 4 * TC_TILES, TC_ISSUE = TC_SOFTMAX_WARPS, TC_LOAD = TC_ISSUE + 1, TC_THREADS = 32 * (TC_LOAD + 1);
+constexpr uint32_t TC_COLS = 512, TC_O_COL = TC_TILES * TC_KEYS;      // S of both tiles, then O of both
+constexpr float TC_SLACK = 20.f;
+
+template <int D>
+struct TcSizes {
+    static constexpr int ATOMS = D / 64, ATOM = 128 * 128;              // 64 features of 128 rows, in bytes
+    static constexpr int TILE = ATOMS * ATOM, STAGES = D == 64 ? 4 : 2;
+    static constexpr size_t SMEM = 1024 + (size_t)(TC_TILES + 2 * STAGES) * TILE;
+};
+
+struct __align__(8) TcSync {
+    uint64_t k_full[4], v_full[4], k_free[4], v_free[4], s_full[TC_TILES], p_ready[TC_TILES], done;
+    uint32_t tmem, failed;
+};
+
+// 32 lanes x 16 columns of 32-bit numbers.
+__device__ __forceinline__ void tmem_load_16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_store_16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+                 ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+                 : "memory");
+}
+
+// D[tmem] (+)= A[tmem] B, A's bfloat16 numbers two a column.
+__device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+template <int D>
+__global__ void __launch_bounds__(TC_THREADS, 1)
+attention_shared_tc_kernel(SharedArgs a, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                           int box_rows, int* __restrict__ status) {
+    using Z = TcSizes<D>;
+    constexpr int STAGES = Z::STAGES, ATOMS = Z::ATOMS;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ TcSync sync;
+    uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t* const q_tiles = smem;
+    uint8_t* const k_tiles = q_tiles + TC_TILES * Z::TILE;
+    uint8_t* const v_tiles = k_tiles + STAGES * Z::TILE;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int kv_head = blockIdx.y, share = a.n_head / a.n_kv_head;
+    Item it;
+    if (!item_of(a, blockIdx.x, nullptr, it)) return;                   // (shared ranges only: the grid has no others)
+    const int n_blocks = (it.key1 - it.key0 + TC_KEYS - 1) / TC_KEYS, pairs = it.rows * share;
+    const int boxes = TC_KEYS / box_rows, box_shift = __ffs(box_rows) - 1;       // (a power of two)
+    // page of box `lane` of a block, -1: none (its keys are not there)
+    auto page_of = [&](int block) {
+        const int position = it.key0 + block * TC_KEYS + lane * box_rows, pi = position / a.page_tokens;
+        int page = lane < boxes && position < it.key1 && pi < a.max_pages ? it.table[pi] : -1;
+        if (page >= 0 && !MG_GUARDED(attention_shared, MG_GUARD_PAGE, page, a.num_pages)) page = -1;
+        return page < a.num_pages ? page : -1;
+    };
+
+    if (tid == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(smem_u32(&sync.k_full[s]), 1);
+            mbar_init(smem_u32(&sync.v_full[s]), 1);
+            mbar_init(smem_u32(&sync.k_free[s]), 1);
+            mbar_init(smem_u32(&sync.v_free[s]), 1);
+        }
+        for (int i = 0; i < TC_TILES; ++i) {
+            mbar_init(smem_u32(&sync.s_full[i]), 1);
+            mbar_init(smem_u32(&sync.p_ready[i]), 128);
+        }
+        mbar_init(smem_u32(&sync.done), 1);
+        sync.failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == TC_ISSUE) tmem_alloc(smem_u32(&sync.tmem), TC_COLS);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sync.tmem;
+    bool good = true;
+    int phase0 = 0;                                                     // blocks of earlier rounds (the barriers go on counting)
+
+    for (int q0 = it.tile * TC_TILES * TC_PAIRS, round = 0; q0 < pairs; q0 += it.tiles * TC_TILES * TC_PAIRS, ++round) {
+        const int n_tiles = pairs - q0 > TC_PAIRS ? 2 : 1;
+        // queries: a pair a row of the tile, swizzled; pairs that are not there are zeros
+        for (int i = tid; i < n_tiles * TC_PAIRS * (D / 8); i += TC_THREADS) {
+            const int j = i / (D / 8), c = i % (D / 8), row = pair_row(a, it, q0 + j, share);
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (row >= 0)
+                v = *reinterpret_cast<const uint4*>((const bf16*)a.q + row * a.q_stride + (size_t)(kv_head * share + (q0 + j) % share) * D + c * 8);
+            *reinterpret_cast<uint4*>(q_tiles + (j / TC_PAIRS) * Z::TILE + (c / 8) * Z::ATOM + (j % TC_PAIRS) * 128 +
+                                      (((c % 8) ^ (j & 7)) * 16)) = v;
+        }
+        async_proxy_fence();
+        __syncthreads();
+
+        if (warp == TC_LOAD) {
+            int code = 0;
+            for (int j = 0; j < n_blocks; ++j) {
+                const int page = page_of(j), n = phase0 + j, stage = n % STAGES;
+                const int position = it.key0 + j * TC_KEYS + lane * box_rows;
+                // (no page: rows in front of the pool, which the copy fills with zeros)
+                const int y = page < 0 ? -box_rows : (page * a.n_kv_head + kv_head) * a.page_tokens + position % a.page_tokens;
+#pragma unroll
+                for (int which = 0; which < 2; ++which) {
+                    uint64_t* const full = which ? &sync.v_full[stage] : &sync.k_full[stage];
+                    uint64_t* const free = which ? &sync.v_free[stage] : &sync.k_free[stage];
+                    if (n >= STAGES && !warp_wait(smem_u32(free), (n / STAGES - 1) & 1)) { code = 60; break; }
+                    if (lane == 0) mbar_expect_tx(smem_u32(full), Z::TILE);
+                    __syncwarp();
+                    if (lane < boxes)
+#pragma unroll
+                        for (int atom = 0; atom < ATOMS; ++atom)
+                            tma_load_2d(smem_u32((which ? v_tiles : k_tiles) + stage * Z::TILE + atom * Z::ATOM + lane * box_rows * 128),
+                                        which ? &map_v : &map_k, smem_u32(full), atom * 64, y);
+                    __syncwarp();
+                }
+                if (code) break;
+            }
+            if (code) {
+                if (lane == 0) { atomicExch(status, code); *(volatile uint32_t*)&sync.failed = 1; }
+                good = false;
+            }
+        } else if (warp == TC_ISSUE) {
+            auto scores = [&](int j, int i) {                           // S_i(j) = Q_i K(j)^T
+                const int n = phase0 + j, stage = n % STAGES;
+                if (i == 0 && !warp_wait(smem_u32(&sync.k_full[stage]), (n / STAGES) & 1)) return false;
+                tc_fence_after();
+                if (elect_one()) {
+                    constexpr uint32_t idesc = instr_desc_bf16(TC_PAIRS, TC_KEYS, false);
+                    const uint64_t dq = smem_desc_sw128(smem_u32(q_tiles + i * Z::TILE)), dk = smem_desc_sw128(smem_u32(k_tiles + stage * Z::TILE));
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k) {
+                        const uint64_t step = (uint64_t)((k / 4 * Z::ATOM + k % 4 * 32) >> 4);
+                        umma_bf16(tmem + i * TC_KEYS, dq + step, dk + step, idesc, k ? 1u : 0u);
+                    }
+                    umma_commit(smem_u32(&sync.s_full[i]));
+                    if (i == n_tiles - 1) umma_commit(smem_u32(&sync.k_free[stage]));
+                }
+                __syncwarp();
+                return true;
+            };
+            int code = 0;
+            for (int i = 0; i < n_tiles && code == 0; ++i)
+                if (!scores(0, i)) code = 61;
+            for (int j = 0; j < n_blocks && code == 0; ++j) {
+                const int n = phase0 + j, stage = n % STAGES;
+                for (int i = 0; i < n_tiles && code == 0; ++i) {
+                    if (!warp_wait(smem_u32(&sync.p_ready[i]), n & 1)) { code = 62; break; }
+                    if (i == 0 && !warp_wait(smem_u32(&sync.v_full[stage]), (n / STAGES) & 1)) { code = 63; break; }
+                    tc_fence_after();
+                    if (elect_one()) {
+                        constexpr uint32_t idesc = instr_desc_bf16(TC_PAIRS, 64, true);
+#pragma unroll
+                        for (int atom = 0; atom < ATOMS; ++atom)
+#pragma unroll
+                            for (int k = 0; k < TC_KEYS / 16; ++k)
+                                umma_bf16_ts(tmem + TC_O_COL + i * D + atom * 64, tmem + i * TC_KEYS + k * 8,
+                                             smem_desc_sw128(smem_u32(v_tiles + stage * Z::TILE + atom * Z::ATOM + k * (16 * 128))), idesc,
+                                             (j | k) ? 1u : 0u);
+                        if (i == n_tiles - 1) {
+                            umma_commit(smem_u32(&sync.v_free[stage]));
+                            if (j == n_blocks - 1) umma_commit(smem_u32(&sync.done));
+                        }
+                    }
+                    __syncwarp();
+                    // (in order behind the product that reads P in S's place)
+                    if (j + 1 < n_blocks && !scores(j + 1, i)) code = 61;
+                }
+            }
+            if (code) {
+                if (lane == 0) { atomicExch(status, code); *(volatile uint32_t*)&sync.failed = 1; }
+                good = false;
+            }
+        } else {
+            const int i = warp / 4, j = q0 + i * TC_PAIRS + (tid & 127);
+            if (i < n_tiles) {
+                const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), s_at = lanes + i * TC_KEYS, o_at = lanes + TC_O_COL + i * D;
+                float ref = -INFINITY, total = 0.f;
+                int page = page_of(0);
+                for (int b = 0; b < n_blocks; ++b) {
+                    const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
+                    if (b + 1 < n_blocks) page = page_of(b + 1);
+                    const int n = phase0 + b, stage = n % STAGES, last = it.key1 - it.key0 - b * TC_KEYS;     // keys of this block
+                    if (!warp_wait(smem_u32(&sync.s_full[i]), n & 1)) { good = false; atomicExch(status, 64); break; }
+                    tc_fence_after();
+                    uint32_t s[TC_KEYS];
+#pragma unroll
+                    for (int c = 0; c < TC_KEYS / 32; ++c) tmem_load_32(s_at + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
+                    tmem_wait_ld();
+                    if (last < TC_KEYS || there != (uint32_t)((1ull << boxes) - 1)) {
+#pragma unroll
+                        for (int c = 0; c < TC_KEYS; ++c)
+                            if (c >= last || !((there >> (c >> box_shift)) & 1u)) s[c] = 0xff800000u;
+                    }
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int c = 0; c < TC_KEYS; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(s[c]));
+                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2e;
+                    const bool high = top > ref + TC_SLACK;             // (also the first block that has a key at all)
+                    if (__any_sync(0xffffffffu, high)) {
+                        float corr = 1.f;
+                        if (high) {
+                            corr = ref == -INFINITY ? 0.f : exp2f(ref - top);
+                            ref = top;
+                        }
+                        total *= corr;
+                        if (b > 0) {                                    // (the products before this block's scores are over)
+#pragma unroll
+                            for (int c = 0; c < D / 16; ++c) {
+                                uint32_t r[16];
+                                tmem_load_16(o_at + c * 16, r);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int k = 0; k < 16; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * corr);
+                                tmem_store_16(o_at + c * 16, r);
+                            }
+                        }
+                    }
+                    const float shift = ref == -INFINITY ? 0.f : ref;
+                    float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        uint32_t p[16];
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) {
+                            const float e0 = exp2_approx(fmaf(__uint_as_float(s[h * 32 + 2 * c]), a.scale_log2e, -shift));
+                            const float e1 = exp2_approx(fmaf(__uint_as_float(s[h * 32 + 2 * c + 1]), a.scale_log2e, -shift));
+                            part[c & 3] += e0 + e1;
+                            p[c] = pack_bf16(e0, e1);
+                        }
+                        tmem_store_16(s_at + h * 16, p);
+                    }
+                    total += (part[0] + part[1]) + (part[2] + part[3]);
+                    // value rows behind the range's last key hold whatever is in the page: 0 times that has to be 0
+                    if (last < TC_KEYS && i == 0) {
+                        if (!warp_wait(smem_u32(&sync.v_full[stage]), (n / STAGES) & 1)) { good = false; atomicExch(status, 65); break; }
+                        if (tid >= last)
+#pragma unroll
+                            for (int atom = 0; atom < ATOMS; ++atom)
+#pragma unroll
+                                for (int c = 0; c < 8; ++c)
+                                    *reinterpret_cast<uint4*>(v_tiles + stage * Z::TILE + atom * Z::ATOM + tid * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+                        async_proxy_fence();
+                    }
+                    tmem_wait_st();
+                    tc_fence_before();
+                    mbar_arrive(smem_u32(&sync.p_ready[i]));
+                }
+                if (good && !warp_wait(smem_u32(&sync.done), round & 1)) { good = false; atomicExch(status, 66); }
+                tc_fence_after();
+                const int row = pair_row(a, it, j, share);
+                const bool failed = !good || *(volatile uint32_t*)&sync.failed != 0;
+                const size_t at = ((size_t)max(row, 0) * a.n_head + kv_head * share + j % share) * (a.shared_slots + a.own_slots) + it.slot;
+                float4* const dst = reinterpret_cast<float4*>(a.part_out + at * D);
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t r[32];
+                    tmem_load_32(o_at + c * 32, r);
+                    tmem_wait_ld();
+                    if (row >= 0 && !failed)
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            dst[c * 8 + k] = make_float4(__uint_as_float(r[4 * k]), __uint_as_float(r[4 * k + 1]), __uint_as_float(r[4 * k + 2]),
+                                                         __uint_as_float(r[4 * k + 3]));
+                }
+                if (row >= 0 && !failed) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(ref, total);
+            }
+        }
+        tc_fence_before();
+        good = __syncthreads_and(good) && *(volatile uint32_t*)&sync.failed == 0;
+        tc_fence_after();
+        if (!good) break;
+        phase0 += n_blocks;
+    }
+    if (!good && tid == 0)
+        for (int i = 0; i < 2000; ++i) __nanosleep(1000);               // let copies in flight land
+    __syncthreads();
+    if (warp == TC_ISSUE) tmem_dealloc(tmem, TC_COLS);
+}
+
 // ---- the ranges of a (row, head) joined: a warp each ------------------------------------------------------------------
 template <typename T>
 __global__ void __launch_bounds__(128) attention_shared_join_kernel(SharedArgs a) {
@@ -514,7 +819,7 @@ __global__ void __launch_bounds__(128) attention_shared_join_kernel(SharedArgs a
         for (int d = lane; d < a.D; d += 32) out[d] = from_float<T>(0.f);
         return;
     }
-    const int shared_step = range_keys(behind, a.shared_slots, SHARED_LEAST), own = p + 1 - behind;
+    const int shared_step = range_keys(behind, a.shared_slots, a.shared_least), own = p + 1 - behind;
     const int own_step = range_keys(own, a.own_slots, OWN_LEAST);
     const int n_shared = (behind + shared_step - 1) / shared_step, n_all = n_shared + (own + own_step - 1) / own_step;
     const size_t base = ((size_t)row * a.n_head + head) * (a.shared_slots + a.own_slots);
@@ -551,11 +856,28 @@ template <typename... KArgs>
 int launch_ranges(void (*kernel)(KArgs...), int threads, size_t smem, const SharedArgs& a, cudaStream_t s) {
     const cudaError_t e = mg_raise_shared(kernel, smem);
     if (e != cudaSuccess) return mg_set_error(MG_ERR_CUDA, "attention (shared): cannot raise shared memory: %s", cudaGetErrorString(e));
-    const long long items = (long long)a.n_groups * a.row_tiles * a.shared_slots + (long long)a.n * a.own_slots;
+    const long long items = (long long)a.n_groups * a.row_tiles * a.shared_slots + (long long)a.n * a.own_slots - a.first_item;
     kernel<<<dim3((unsigned)items, a.n_kv_head), threads, smem, s>>>(a);
     MG_CHECK_LAUNCH("attention (shared)");
     return MG_OK;
 }
+
+template <int D>
+int launch_tc(const SharedArgs& a, int* status, cudaStream_t s) {
+    const int box_rows = a.page_tokens < TC_KEYS ? a.page_tokens : TC_KEYS;
+    CUtensorMap map_k, map_v;
+    int rc = tensor_map(a.k_pages, a.num_pages * a.n_kv_head * a.page_tokens, D, box_rows, &map_k);
+    if (rc == MG_OK) rc = tensor_map(a.v_pages, a.num_pages * a.n_kv_head * a.page_tokens, D, box_rows, &map_v);
+    if (rc != MG_OK) return rc;
+    const cudaError_t e = mg_raise_shared(attention_shared_tc_kernel<D>, TcSizes<D>::SMEM);
+    if (e != cudaSuccess) return mg_set_error(MG_ERR_CUDA, "attention (shared): cannot raise shared memory: %s", cudaGetErrorString(e));
+    attention_shared_tc_kernel<D><<<dim3((unsigned)(a.n_groups * a.row_tiles * a.shared_slots), a.n_kv_head), TC_THREADS, TcSizes<D>::SMEM, s>>>(
+        a, map_k, map_v, box_rows, status);
+    MG_CHECK_LAUNCH("attention (shared, tcgen05)");
+    return MG_OK;
+}
+
+constexpr int TC_LEAST_PAIRS = 64;
 
 template <int DP>
 int launch_mma(const SharedArgs& a, int pair_tiles, cudaStream_t s) {
@@ -570,24 +892,35 @@ int launch_mma(const SharedArgs& a, int pair_tiles, cudaStream_t s) {
 
 int padded_head(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
+// Where the maxima and sums lie behind the averages in the scratch, in floats (pairs of them are read at once).
+size_t sums_at(size_t slots, int head_dim) { return (slots * head_dim + 3) / 4 * 4; }
+
 // How a launch is cut.
 struct Cut {
-    bool mma;            // the warp-level tensor cores, or 32-bit arithmetic
+    bool mma, tc;        // the warp-level tensor cores; shared ranges on tcgen05
     int pair_tiles;      // mma: tiles of 8 pairs that a CTA takes at once
     int row_tiles;       // CTAs that share the pairs of a group
     int shared_slots, own_slots;      // ranges of shared keys, and of a row's own
+    int shared_least;
 };
-Cut cut(int n_groups, int max_rows, int max_tokens, int max_behind, int n, int n_head, int n_kv_head, int head_dim, bool is_bf16) {
+Cut cut(int n_groups, int max_rows, int max_tokens, int max_behind, int n, int n_head, int n_kv_head, int head_dim, int page_tokens,
+        bool is_bf16) {
     Cut c;
     const int share = n_head / n_kv_head, pairs = n_groups > 0 ? (max_rows < n ? max_rows : n) * share : share;
     c.mma = is_bf16 && head_dim % 8 == 0;
+    c.tc = n_groups > 0 && is_bf16 && (head_dim == 64 || head_dim == 128) && pairs >= TC_LEAST_PAIRS && page_tokens % 8 == 0 &&
+           (page_tokens < TC_KEYS ? TC_KEYS % page_tokens == 0 : page_tokens % TC_KEYS == 0) && max_tokens >= TC_KEYS;
     const int most_tiles = head_dim <= 64 ? 4 : head_dim <= 128 ? 2 : 1;      // what the registers hold
-    c.pair_tiles = pairs <= 8 ? 1 : pairs <= 16 && most_tiles > 1 ? 2 : most_tiles;
-    c.row_tiles = ceil_div(pairs, c.mma ? 8 * c.pair_tiles : SIMT_QUERIES);
+    const int mma_pairs = c.tc ? share : pairs;
+    c.pair_tiles = mma_pairs <= 8 ? 1 : mma_pairs <= 16 && most_tiles > 1 ? 2 : most_tiles;
+    c.row_tiles = ceil_div(pairs, c.tc ? TC_TILES * TC_PAIRS : c.mma ? 8 * c.pair_tiles : SIMT_QUERIES);
+    c.shared_least = c.tc ? TC_KEYS : BLOCK_KEYS;
     const long long shared_ctas = (long long)n_groups * c.row_tiles * n_kv_head, own_ctas = (long long)n * n_kv_head;
-    const int most_shared = ceil_div(max_tokens > 0 ? max_tokens : 1, SHARED_LEAST), most_own = ceil_div(max_behind, OWN_LEAST);
+    const int most_shared = ceil_div(max_tokens > 0 ? max_tokens : 1, c.shared_least), most_own = ceil_div(max_behind, OWN_LEAST);
     const long long want = 148 * 4;
-    const long long x = shared_ctas > 0 ? (want + shared_ctas - 1) / shared_ctas : 1, y = (want + own_ctas - 1) / own_ctas;
+    long long x = shared_ctas > 0 ? (want + shared_ctas - 1) / shared_ctas : 1;
+    if (c.tc) x = 148 / shared_ctas;                       // one CTA an SM
+    const long long y = (want + own_ctas - 1) / own_ctas;
     c.shared_slots = (int)(x < 1 ? 1 : x > most_shared ? most_shared : x);
     c.own_slots = (int)(y < 1 ? 1 : y > most_own ? most_own : y);
     return c;
@@ -597,10 +930,17 @@ Cut cut(int n_groups, int max_rows, int max_tokens, int max_behind, int n, int n
 
 // Floats of scratch that mg_attention_shared() takes for these sizes and bounds.
 MG_API long long mg_attention_shared_scratch_floats(int n_groups, int max_rows, int max_tokens, int max_behind, int n, int n_head,
-                                                    int n_kv_head, int head_dim, int is_bf16) {
-    if (n_groups < 0 || max_rows <= 0 || n <= 0 || n_head <= 0 || n_kv_head <= 0 || n_head % n_kv_head != 0 || max_behind <= 0) return 0;
-    const Cut c = cut(n_groups, max_rows, max_tokens, max_behind, n, n_head, n_kv_head, head_dim, is_bf16 != 0);
-    return (long long)n * n_head * (c.shared_slots + c.own_slots) * (head_dim + 2);
+                                                    int n_kv_head, int head_dim, int page_tokens, int is_bf16) {
+    if (n_groups < 0 || max_rows <= 0 || n <= 0 || n_head <= 0 || n_kv_head <= 0 || n_head % n_kv_head != 0 || max_behind <= 0 || page_tokens <= 0) return 0;
+    const Cut c = cut(n_groups, max_rows, max_tokens, max_behind, n, n_head, n_kv_head, head_dim, page_tokens, is_bf16 != 0);
+    const size_t slots = (size_t)n * n_head * (c.shared_slots + c.own_slots);
+    return (long long)(sums_at(slots, head_dim) + 2 * slots);
+}
+
+MG_API int mg_attention_shared_launches(int n_groups, int max_rows, int max_tokens, int max_behind, int n, int n_head, int n_kv_head,
+                                        int head_dim, int page_tokens, int is_bf16) {
+    if (n <= 0 || max_rows <= 0 || n_kv_head <= 0 || n_head % n_kv_head != 0 || max_behind <= 0 || page_tokens <= 0) return 0;
+    return cut(n_groups, max_rows, max_tokens, max_behind, n, n_head, n_kv_head, head_dim, page_tokens, is_bf16 != 0).tc ? 3 : 2;
 }
 
 // Attention of n single query tokens, groups of which share their first keys.  q: rows of q_stride elements whose first
@@ -610,12 +950,13 @@ MG_API long long mg_attention_shared_scratch_floats(int n_groups, int max_rows, 
 // same keys and values over the shared tokens.  max_rows, max_tokens, max_behind: how many rows a group has, how many
 // tokens it shares and how many keys a row has besides, at most (bounds that are too low cost time).  A row whose position
 // is below zero is padding: its output is zeros.  scratch: mg_attention_shared_scratch_floats() floats, 16-byte aligned,
-// that no other launch uses meanwhile.  Two launches.  MG_ERR_UNSUPPORTED for heads of more than 256 features.
+// that no other launch uses meanwhile.  status: a word that gets a code if a bounded wait runs out.  mg_attention_shared_launches()
+// launches.  MG_ERR_UNSUPPORTED for heads of more than 256 features.
 MG_API int mg_attention_shared(const void* q, long long q_stride, const void* k_pages, const void* v_pages, const int* table,
                                const int* token_request, const int* positions, const int* groups, int n_groups, int max_rows,
                                int max_tokens, int max_behind, void* out, float* scratch, int n, int n_head, int n_kv_head,
                                int head_dim, int page_tokens, int max_pages, int num_pages, int n_requests, float scale,
-                               int is_bf16, void* stream) {
+                               int is_bf16, int* status, void* stream) {
     if (n == 0) return MG_OK;
     MG_REQUIRE(n > 0 && n_head > 0 && n_kv_head > 0 && head_dim > 0 && page_tokens > 0 && max_pages > 0 && num_pages > 0 && n_requests > 0,
                "attention (shared): bad sizes");
@@ -627,22 +968,28 @@ MG_API int mg_attention_shared(const void* q, long long q_stride, const void* k_
     if (head_dim > 256 || n_kv_head > 65535)
         return mg_set_error(MG_ERR_UNSUPPORTED, "attention (shared): head_dim %d is more than 256", head_dim);
     SharedArgs a;
-    const Cut c = cut(n_groups, max_rows, max_tokens, max_behind, n, n_head, n_kv_head, head_dim, is_bf16 != 0);
+    const Cut c = cut(n_groups, max_rows, max_tokens, max_behind, n, n_head, n_kv_head, head_dim, page_tokens, is_bf16 != 0);
     a.q = q; a.q_stride = q_stride; a.k_pages = k_pages; a.v_pages = v_pages; a.table = table; a.token_request = token_request;
     a.positions = positions; a.groups = groups; a.out = out;
     a.n_groups = n_groups; a.n = n; a.n_head = n_head; a.n_kv_head = n_kv_head; a.D = head_dim; a.page_tokens = page_tokens;
     a.max_pages = max_pages; a.num_pages = num_pages; a.n_requests = n_requests;
+    a.first_item = 0; a.shared_least = c.shared_least;
     a.row_tiles = c.row_tiles; a.shared_slots = c.shared_slots; a.own_slots = c.own_slots;
     a.scale_log2e = scale * 1.4426950408889634f;
     const size_t slots = (size_t)n * n_head * (c.shared_slots + c.own_slots);
-    a.part_ml = scratch;
-    a.part_out = scratch + 2 * slots;
+    a.part_out = scratch;
+    a.part_ml = scratch + sums_at(slots, head_dim);
     const long long items = (long long)n_groups * c.row_tiles * c.shared_slots + (long long)n * c.own_slots;
     MG_REQUIRE(items < (1ll << 31), "attention (shared): too many rows");
     cudaStream_t s = (cudaStream_t)stream;
     int rc;
     if (c.mma && ((((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages) & 15) || q_stride % 2))
         return mg_set_error(MG_ERR_ARG, "attention (shared): queries and pages have to be 16-byte aligned, rows of queries 4-byte aligned");
+    if (c.tc) {
+        rc = head_dim == 64 ? launch_tc<64>(a, status, s) : launch_tc<128>(a, status, s);
+        if (rc != MG_OK) return rc;
+        a.first_item = n_groups * c.row_tiles * c.shared_slots;         // what is left are the rows' own ranges
+    }
     if (c.mma) {
         switch (padded_head(head_dim)) {
             case 32: rc = launch_mma<32>(a, c.pair_tiles, s); break;

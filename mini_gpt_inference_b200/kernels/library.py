@@ -103,7 +103,8 @@ _SIGNATURES = {
     "mg_attention_prefill_tc": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I,
                                 ctypes.c_longlong, _I, _I, _F, _I, _I, _P, _I, _P, _P],
     "mg_attention_shared": [_P, ctypes.c_longlong, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I,
-                            _F, _I, _P],
+                            _F, _I, _P, _P],
+    "mg_attention_shared_launches": [_I] * 10,
     "mg_beam_select": [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, ctypes.c_double, _P, _P, _P, _P, _P, _P, _P, _P],
     "mg_beam_reorder": [_P, _P, _P, _I, _I, _P, _P, _P, _P, _I, _P, _P, _P, _P],
     "mg_step_tables": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P],
@@ -173,7 +174,7 @@ def load(verbose: bool = True):
     lib.mg_attention_mma_scratch_floats.restype = ctypes.c_longlong
     lib.mg_attention_split_scratch_floats.argtypes = [c_int, c_int, c_int, c_int]
     lib.mg_attention_split_scratch_floats.restype = ctypes.c_longlong
-    lib.mg_attention_shared_scratch_floats.argtypes = [c_int] * 9
+    lib.mg_attention_shared_scratch_floats.argtypes = [c_int] * 10
     lib.mg_attention_shared_scratch_floats.restype = ctypes.c_longlong
     lib.mg_beam_select_scratch_bytes.argtypes = [c_int] * 4
     lib.mg_beam_select_scratch_bytes.restype = ctypes.c_longlong

@@ -988,13 +988,14 @@ class CudaOps:
         if n == 0:
             return out
         sizes = (groups.shape[0], int(shared.max_rows), int(shared.max_tokens), int(shared.max_behind))
-        floats = self.lib.mg_attention_shared_scratch_floats(*sizes, n, n_head, n_kv_head, head_dim, is_bf16)
+        shape = (*sizes, n, n_head, n_kv_head, head_dim, cache.page_tokens, is_bf16)
+        floats = self.lib.mg_attention_shared_scratch_floats(*shape)
         scratch = torch.empty((floats,), dtype=torch.float32, device=self.device)
         self._run(self.lib.mg_attention_shared(
             _ptr(qkv), qkv.shape[1], _ptr(k), _ptr(v), _ptr(table), _ptr(ctx.token_request), _ptr(ctx.positions), _ptr(groups),
             *sizes, _ptr(out), _ptr(scratch), n, n_head, n_kv_head, head_dim, cache.page_tokens, table.shape[1], k.shape[0],
-            table.shape[0], float(scale), is_bf16, self._stream()), "paged_attention (shared)")
-        self.launches += 1                                       # the ranges joined
+            table.shape[0], float(scale), is_bf16, _ptr(self.status), self._stream()), "paged_attention (shared)")
+        self.launches += self.lib.mg_attention_shared_launches(*shape) - 1
         return out
 
     def head_prepare(self, proj, n_head, n_kv_head, head_dim, v_dim, q_off, k_off, v_off, unit_norm, eps,

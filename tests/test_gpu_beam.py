@@ -125,6 +125,26 @@ def test_attention_shared(ops, dtype, shape, heads, page):
     check_attention(case, run_attention(ops, case), dtype)
 
 
+@pytest.mark.parametrize("heads,page,shape", [
+    ((8, 8, 64), 16, [(700, [3] * 70)]), ((32, 8, 128), 64, [(1300, [1 + i % 50 for i in range(100)]), (128, [5] * 3)]),
+    ((16, 2, 128), 8, [(129, [2] * 9), (64, [1] * 20), (400, [-5, 7] * 20)]), ((64, 1, 64), 128, [(2049, [9] * 5), (0, [200] * 2)]),
+    ((12, 4, 64), 32, [(300, [4] * 171)]), ((5, 1, 128), 256, [(513, [3] * 26)]), ((96, 1, 128), 16, [(1000, [70])])])
+@pytest.mark.parametrize("spread", [2.0, 30.0])
+def test_attention_shared_many_pairs(ops, heads, page, shape, spread):
+    """Tiles of 128 (row, head) pairs on the 5th-generation tensor cores: odd numbers of pairs and keys, rows in front of the
+    shared end, scores whose largest come late (the reference moves)."""
+    case = shared_case(shape, [40], heads, page, BF16, seed=21, pad=1, spread=spread)
+    H, KV, D = heads
+    out = run_attention(ops, case)
+    ops.check_status()
+    for r, (k, v) in enumerate(zip(case.k, case.v)):
+        want, size = plain_beam.attention_row(case.q[r, : H * D].cpu().reshape(H, D), k, v, D ** -0.5)
+        # as in check_attention, the scores being `spread` / 2 times as large
+        tol = (20 * spread * math.sqrt(D) * 2.0 ** -24 + 2.0 ** -8) * (size + want.abs()) + 1e-6
+        assert ((out[r].double().cpu().reshape(H, D) - want).abs() <= tol).all(), r
+    assert (out[len(case.k):] == 0).all()
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("bounds", [(1, 1, 1), (1, 0, 1), (3, 10000, 10000), (64, 64, 64)])
 def test_attention_shared_bounds_are_hints(ops, dtype, bounds):
