@@ -36,11 +36,12 @@ struct SharedArgs {
     void* out;                         // [n][n_head * D]
     float* part_out;                   // [row][head][slot][D]
     float* part_ml;                    // [row][head][slot][2]
+    int* behind;                       // [row]: keys that its shared ranges hold (the ranges' kernel tells the joining one)
     int n_groups, n, n_head, n_kv_head, D, page_tokens, max_pages, num_pages, n_requests;
     int row_tiles;                     // CTAs that share the (row, head) pairs of a group
     int shared_slots, own_slots;       // ranges of the shared keys, and of a row's own
     int shared_least;                  // keys of a range of shared keys, at least, and what they are a multiple of
-    int first_item;                    // item of the grid's first CTA
+    int first_item;                    // item of the grid's first CTA: above 0 where another kernel takes the shared ranges
     float scale_log2e;
 };
 
@@ -52,16 +53,23 @@ __device__ __forceinline__ int range_keys(int keys, int slots, int least) {
 
 constexpr int OWN_LEAST = 64;
 
-// The shared tokens of the group that `row` belongs to (0: none), by all threads of a CTA; `hold` is a word of shared memory.
-__device__ __forceinline__ int group_tokens(const SharedArgs& a, int row, int* hold) {
-    if (threadIdx.x == 0) *hold = 0;
-    __syncthreads();
-    for (int g = threadIdx.x; g < a.n_groups; g += blockDim.x) {
-        const int first = a.groups[3 * g], rows = a.groups[3 * g + 1];
-        if (row >= first && row - first < rows) *hold = a.groups[3 * g + 2];
+// The shared tokens of the group that `row` belongs to (0: none); every warp finds them for itself.
+__device__ __forceinline__ int group_tokens(const SharedArgs& a, int row) {
+    const int lane = threadIdx.x & 31;
+    int tokens = 0;
+    for (int g0 = 0; g0 < a.n_groups; g0 += 32) {
+        const int g = g0 + lane;
+        bool mine = false;
+        int shared = 0;
+        if (g < a.n_groups) {
+            const int first = a.groups[3 * g], rows = a.groups[3 * g + 1];
+            shared = a.groups[3 * g + 2];
+            mine = row >= first && row - first < rows;
+        }
+        const uint32_t found = __ballot_sync(0xffffffffu, mine);
+        if (found) tokens = __shfl_sync(0xffffffffu, shared, __ffs(found) - 1);
     }
-    __syncthreads();
-    return *hold;
+    return tokens;
 }
 
 // What a CTA works on: (row, head) pairs of `rows` rows and the keys key0 .. key1 - 1 that their ranges `slot` hold.
@@ -71,13 +79,14 @@ struct Item {
     const int* table;
 };
 
-// False if there is nothing to do.  All threads of the CTA call it.
-__device__ __forceinline__ bool item_of(const SharedArgs& a, int item, int* hold, Item& it) {
+// False if there is nothing to do.  Whole warps call it.
+__device__ __forceinline__ bool item_of(const SharedArgs& a, int item, Item& it) {
     const int shared_items = a.n_groups * a.row_tiles * a.shared_slots;
     it.shared = item < shared_items;
     it.shared_keys = 0;
     it.tile = 0;
     it.tiles = it.rows = 1;
+    int request;
     if (it.shared) {
         it.slot = item % a.shared_slots;
         item /= a.shared_slots;
@@ -89,6 +98,7 @@ __device__ __forceinline__ bool item_of(const SharedArgs& a, int item, int* hold
         it.shared_keys = a.groups[3 * g + 2];
         if (it.first_row < 0 || it.rows <= 0 || it.first_row >= a.n) return false;
         it.rows = min(it.rows, a.n - it.first_row);
+        request = a.token_request[it.first_row];
         const int step = range_keys(it.shared_keys, a.shared_slots, a.shared_least);
         it.key0 = it.slot * step;
         it.key1 = min(it.shared_keys, it.key0 + step);
@@ -97,14 +107,15 @@ __device__ __forceinline__ bool item_of(const SharedArgs& a, int item, int* hold
         it.slot = item % a.own_slots;
         it.first_row = item / a.own_slots;
         const int p = a.positions[it.first_row];
-        int behind = group_tokens(a, it.first_row, hold);
+        request = a.token_request[it.first_row];
+        int behind = group_tokens(a, it.first_row);
         if (behind > p + 1) behind = 0;
+        if (it.slot == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.behind[it.first_row] = behind;
         const int step = range_keys(p + 1 - behind, a.own_slots, OWN_LEAST);
         it.key0 = behind + it.slot * step;
         it.key1 = min(p + 1, it.key0 + step);
         it.slot += a.shared_slots;
     }
-    int request = a.token_request[it.first_row];
     if (!MG_GUARDED(attention_shared, MG_GUARD_REQUEST, request, a.n_requests)) request = 0;
     it.table = a.table + (size_t)request * a.max_pages;
     return it.key0 < it.key1;
@@ -135,7 +146,7 @@ __host__ __device__ constexpr int simt_lanes(int d) { return d > 64 ? 128 : d > 
 template <typename T>
 __global__ void __launch_bounds__(SIMT_THREADS) attention_shared_simt_kernel(SharedArgs a) {
     extern __shared__ float smem[];
-    __shared__ int krow[BLOCK_KEYS], q_token[SIMT_QUERIES], q_head[SIMT_QUERIES], hold;
+    __shared__ int krow[BLOCK_KEYS], q_token[SIMT_QUERIES], q_head[SIMT_QUERIES];
     __shared__ float q_max[SIMT_QUERIES], q_sum[SIMT_QUERIES], q_corr[SIMT_QUERIES];
     const int tid = threadIdx.x, D = a.D, kv_head = blockIdx.y, share = a.n_head / a.n_kv_head;
     float* q_s = smem;                                   // [D][16]
@@ -144,7 +155,9 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_shared_simt_kernel(Sha
     const int lanes = simt_lanes(D), dl = tid % lanes, ks = tid / lanes, key_parts = SIMT_THREADS / lanes;
 
     Item it;
-    if (!item_of(a, a.first_item + blockIdx.x, &hold, it)) return;
+    pdl_wait();
+    pdl_trigger();
+    if (!item_of(a, a.first_item + blockIdx.x, it)) return;
     for (int q0 = it.tile * SIMT_QUERIES; q0 < it.rows * share; q0 += it.tiles * SIMT_QUERIES) {
         __syncthreads();
         if (tid < SIMT_QUERIES) {
@@ -295,7 +308,7 @@ constexpr int MMA_THREADS = 128, MMA_WARPS = MMA_THREADS / 32, UNIT = 16;       
 // Sizes by padded head: DP features (32, 64, 128 or 256), of which D are there and the others zero.
 template <int DP>
 struct MmaSizes {
-    static constexpr int STAGES = DP <= 64 ? 4 : DP == 128 ? 3 : 2;
+    static constexpr int STAGES = DP == 32 ? 4 : DP == 64 ? 3 : 2;
     static constexpr int TILE = UNIT * DP * 2;                          // bytes of 16 keys or values
     static constexpr size_t SMEM = (size_t)MMA_WARPS * STAGES * 2 * TILE;
 };
@@ -308,14 +321,20 @@ __global__ void __launch_bounds__(MMA_THREADS) attention_shared_mma_kernel(Share
     constexpr int PSTRIDE = DP + 2;                                     // floats of a warp's partial: O, maximum, sum
     static_assert((size_t)MMA_WARPS * NT * 8 * PSTRIDE * 4 <= Z::SMEM, "the warps' results meet where the tiles were");
     extern __shared__ __align__(128) uint8_t ring[];
-    __shared__ int hold;
     __shared__ uint32_t valid[MMA_WARPS][STAGES];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int kv_head = blockIdx.y, share = a.n_head / a.n_kv_head, D = a.D, pieces = D / 8;
     const bf16* const k_pages = (const bf16*)a.k_pages;
     const bf16* const v_pages = (const bf16*)a.v_pages;
     Item it;
-    if (!item_of(a, a.first_item + blockIdx.x, &hold, it)) return;
+    // Behind the kernel of the shared ranges this one starts while that still runs: what both read was there before that one
+    // let it start.  It ends behind that one (the joining kernel waits for this kernel alone).
+    if (a.first_item == 0) pdl_wait();
+    pdl_trigger();
+    if (!item_of(a, a.first_item + blockIdx.x, it)) {
+        if (a.first_item > 0) pdl_wait();
+        return;
+    }
     uint8_t* const mine = ring + (size_t)warp * STAGES * 2 * Z::TILE;
     const uint32_t mine_u = (uint32_t)__cvta_generic_to_shared(mine);
     const uint4 zero4 = make_uint4(0u, 0u, 0u, 0u);
@@ -329,7 +348,7 @@ __global__ void __launch_bounds__(MMA_THREADS) attention_shared_mma_kernel(Share
                 *reinterpret_cast<uint4*>(mine + r * ROWB + ((c ^ (((r % UNIT) / RPL) % SWZ)) * 16)) = zero4;
             }
         }
-        // the first units' rows of the pool, then the copies; the row of the unit after the last one asked for is on its way
+        // the first units' rows of the pool, then the copies; the rows of the unit after the last one asked for are on their way
         auto row_of = [&](int n) {                                      // lane i: row of key i of this warp's n-th unit
             return n < my_units ? cache_row(a, it, it.key0 + (warp + n * MMA_WARPS) * UNIT + (lane & 15), kv_head) : -1;
         };
@@ -358,7 +377,7 @@ __global__ void __launch_bounds__(MMA_THREADS) attention_shared_mma_kernel(Share
         };
         int row = row_of(0);
 #pragma unroll
-        for (int n = 0; n < STAGES - 1; ++n) {
+        for (int n = 0; n < STAGES; ++n) {
             const int next = row_of(n + 1);
             load(n, row);
             row = next;
@@ -392,11 +411,9 @@ __global__ void __launch_bounds__(MMA_THREADS) attention_shared_mma_kernel(Share
         const int krow = (lane & 7) + (((lane >> 3) & 1) << 3), kpiece = lane >> 4;
         const int vrow = (lane & 7) + (((lane >> 4) & 1) << 3), vpiece = (lane >> 3) & 1;
         for (int n = 0; n < my_units; ++n) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
-            __syncwarp();                                               // this unit has landed, the one before is used up
-            const int next = row_of(n + STAGES);
-            load(n + STAGES - 1, row);
-            row = next;
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+            __syncwarp();                                               // this unit has landed
+            const int next = row_of(n + STAGES + 1);
             const uint32_t k_at = mine_u + (uint32_t)(n % STAGES) * 2 * Z::TILE, v_at = k_at + Z::TILE;
             const uint32_t there = valid[warp][n % STAGES];
             float s[NT][4];
@@ -457,6 +474,9 @@ __global__ void __launch_bounds__(MMA_THREADS) attention_shared_mma_kernel(Share
                 for (int nt = 0; nt < NT; ++nt)
                     if (nt < nts) mma_bf16(o[nt][dm], f, pb[nt][0], pb[nt][1]);
             }
+            __syncwarp();                                               // the unit is used up
+            load(n + STAGES, row);
+            row = next;
         }
         // the warps' results meet in shared memory
         asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -500,36 +520,41 @@ __global__ void __launch_bounds__(MMA_THREADS) attention_shared_mma_kernel(Share
         }
         __syncthreads();                                                // (the tiles are loaded again for the next pairs)
     }
+    if (a.first_item > 0) pdl_wait();
 }
 
 // ---- bfloat16, heads of 64 or 128, many pairs: the 5th-generation tensor cores --------------------------------------------
-// A CTA takes two tiles of 128 pairs and walks over the keys of its range in blocks of 128, which both tiles multiply with:
+// A CTA takes two tiles of 128 pairs and walks over the keys of its range in blocks of 64, which both tiles multiply with:
 //
 //   load warp       TMA tiles of keys and values from the pages (one copy per page, tensor and 64 features, 128-byte swizzle)
-//                   into a ring of two stages or more
-//   issue warp      S = Q K^T (128 x 128, TMEM), and O += P V (128 x head, TMEM) with P read from TMEM, where it lies in S's
-//                   place.  The tiles take turns: while one's scores are in the softmax, the other's are computed.
-//   softmax warps   four a tile, a thread a pair: its row of S into registers, 2^(s - ref) as bfloat16 back, the 32-bit sum kept.
-//                   `ref` is the first block's maximum and moves only when a score is more than 2^TC_SLACK above it: O is then
-//                   rescaled in TMEM.  (O / sum does not depend on ref; 2^TC_SLACK keeps the numbers in range.)
+//                   into a ring of stages
+//   issue warps     one a tile: S = Q K^T (128 x 64, one of two TMEM buffers), and O += P V (128 x head, TMEM) with P read from
+//                   TMEM, where it lies in S's place.  The scores of a block are computed while the softmax is at the one before.
+//   softmax warps   eight a tile, two threads a pair, each with half of its row of S: into registers, 2^(s - ref) as bfloat16
+//                   back, the 32-bit sum kept.  `ref` is the first block's maximum and moves only when a block's sum is above 2^60
+//                   (or no number): O is then rescaled in TMEM, and the block done again.  (O / sum does not depend on ref while
+//                   the numbers are in range.)
 //
-// What bounds it: at heads of 128 a block of 128 keys is 2 x 128 x 128 x 128 multiply-adds per product and tile, 1,024 cycles
-// of the tensor core for both, and 16,384 exponentials, 1,024 cycles of the special-function units.  All waits are bounded:
-// when one runs out, `status` gets a code, the CTA writes nothing more, frees its TMEM and returns.
-constexpr int TC_KEYS = 128, TC_PAIRS = 128, TC_TILES = 2;
-constexpr int TC_SOFTMAX_WARPS = 4 * TC_TILES, TC_ISSUE = TC_SOFTMAX_WARPS, TC_LOAD = TC_ISSUE + 1, TC_THREADS = 32 * (TC_LOAD + 1);
-constexpr uint32_t TC_COLS = 512, TC_O_COL = TC_TILES * TC_KEYS;      // S of both tiles, then O of both
-constexpr float TC_SLACK = 20.f;
+// What bounds it: at heads of 128 a block is 2 x 128 x 64 x 128 multiply-adds a tile, 512 cycles of the tensor core (more for S,
+// whose operands are both read from shared memory), and 8,192 exponentials, 512 cycles of the special-function units.  All waits
+// for the tensor core and for copies are bounded: when one runs out, `status` gets a code, the CTA writes nothing more, frees
+// its TMEM and returns.  (Blocks of 128 keys with one buffer a tile, a tile's softmax and products one after the other: 95 us
+// where this takes 88 for 256 rows of 16,384 keys and 32/8 heads of 128.)
+constexpr int TC_KEYS = 64, TC_PAIRS = 128, TC_TILES = 2;
+constexpr int TC_SOFTMAX_WARPS = 8 * TC_TILES, TC_ISSUE = TC_SOFTMAX_WARPS, TC_LOAD = TC_ISSUE + TC_TILES, TC_THREADS = 32 * (TC_LOAD + 1);
+constexpr uint32_t TC_COLS = 512, TC_O_COL = TC_TILES * 2 * TC_KEYS;      // S of both tiles and buffers, then O of both
+constexpr float TC_LIMIT = 1.152921504606846976e18f;                     // 2^60: a block's sum above it moves the reference
 
 template <int D>
 struct TcSizes {
-    static constexpr int ATOMS = D / 64, ATOM = 128 * 128;              // 64 features of 128 rows, in bytes
-    static constexpr int TILE = ATOMS * ATOM, STAGES = D == 64 ? 4 : 2;
-    static constexpr size_t SMEM = 1024 + (size_t)(TC_TILES + 2 * STAGES) * TILE;
+    static constexpr int ATOMS = D / 64, Q_ATOM = TC_PAIRS * 128, ATOM = TC_KEYS * 128;      // 64 features of a tile's rows, in bytes
+    static constexpr int Q_TILE = ATOMS * Q_ATOM, TILE = ATOMS * ATOM, STAGES = 4;
+    static constexpr size_t SMEM = 1024 + (size_t)TC_TILES * Q_TILE + (size_t)2 * STAGES * TILE;
 };
 
 struct __align__(8) TcSync {
-    uint64_t k_full[4], v_full[4], k_free[4], v_free[4], s_full[TC_TILES], p_ready[TC_TILES], done;
+    uint64_t k_full[4], v_full[4], k_free[4], v_free[4], s_full[TC_TILES][2], p_ready[TC_TILES][2], pv_done[TC_TILES], q_ready[TC_TILES], round_done[TC_TILES];
+    float meet[TC_TILES][2][TC_PAIRS];      // what the two threads of a pair tell each other
     uint32_t tmem, failed;
 };
 
@@ -540,11 +565,14 @@ __device__ __forceinline__ void tmem_load_16(uint32_t taddr, uint32_t (&r)[16]) 
                    "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(taddr) : "memory");
 }
-__device__ __forceinline__ void tmem_store_16(uint32_t taddr, const uint32_t (&r)[16]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
-                 ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
-                 : "memory");
+// ... and 8.
+__device__ __forceinline__ void tmem_load_8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_store_8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};"
+                 ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr) : "memory");
 }
 
 // D[tmem] (+)= A[tmem] B, A's bfloat16 numbers two a column.
@@ -567,18 +595,19 @@ attention_shared_tc_kernel(SharedArgs a, const __grid_constant__ CUtensorMap map
     __shared__ TcSync sync;
     uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t* const q_tiles = smem;
-    uint8_t* const k_tiles = q_tiles + TC_TILES * Z::TILE;
+    uint8_t* const k_tiles = q_tiles + TC_TILES * Z::Q_TILE;
     uint8_t* const v_tiles = k_tiles + STAGES * Z::TILE;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // (told by one lane to all: the compiler then knows that the warp agrees, which the tensor core's operands have to)
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int kv_head = blockIdx.y, share = a.n_head / a.n_kv_head;
     Item it;
-    if (!item_of(a, blockIdx.x, nullptr, it)) return;                   // (shared ranges only: the grid has no others)
+    pdl_wait();                                                         // (before the next kernel may start: see there)
+    pdl_trigger();
+    if (!item_of(a, blockIdx.x, it)) return;                   // (shared ranges only: the grid has no others)
     const int n_blocks = (it.key1 - it.key0 + TC_KEYS - 1) / TC_KEYS, pairs = it.rows * share;
     const int boxes = TC_KEYS / box_rows, box_shift = __ffs(box_rows) - 1;       // (a power of two)
-    // page of box `lane` of a block, -1: none (its keys are not there)
-    auto page_of = [&](int block) {
-        const int position = it.key0 + block * TC_KEYS + lane * box_rows, pi = position / a.page_tokens;
-        int page = lane < boxes && position < it.key1 && pi < a.max_pages ? it.table[pi] : -1;
+    auto page_at = [&](int column) {                                    // -1: none (its keys are not there)
+        int page = column < a.max_pages ? it.table[column] : -1;
         if (page >= 0 && !MG_GUARDED(attention_shared, MG_GUARD_PAGE, page, a.num_pages)) page = -1;
         return page < a.num_pages ? page : -1;
     };
@@ -587,14 +616,18 @@ attention_shared_tc_kernel(SharedArgs a, const __grid_constant__ CUtensorMap map
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(smem_u32(&sync.k_full[s]), 1);
             mbar_init(smem_u32(&sync.v_full[s]), 1);
-            mbar_init(smem_u32(&sync.k_free[s]), 1);
-            mbar_init(smem_u32(&sync.v_free[s]), 1);
+            mbar_init(smem_u32(&sync.k_free[s]), TC_TILES);
+            mbar_init(smem_u32(&sync.v_free[s]), TC_TILES);
         }
         for (int i = 0; i < TC_TILES; ++i) {
-            mbar_init(smem_u32(&sync.s_full[i]), 1);
-            mbar_init(smem_u32(&sync.p_ready[i]), 128);
+            mbar_init(smem_u32(&sync.pv_done[i]), 1);
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(smem_u32(&sync.s_full[i][b]), 1);
+                mbar_init(smem_u32(&sync.p_ready[i][b]), 256);
+            }
+            mbar_init(smem_u32(&sync.q_ready[i]), 256);
+            mbar_init(smem_u32(&sync.round_done[i]), 1);
         }
-        mbar_init(smem_u32(&sync.done), 1);
         sync.failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -602,254 +635,370 @@ attention_shared_tc_kernel(SharedArgs a, const __grid_constant__ CUtensorMap map
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = sync.tmem;
-    bool good = true;
-    int phase0 = 0;                                                     // blocks of earlier rounds (the barriers go on counting)
+    const uint32_t tmem = __shfl_sync(0xffffffffu, sync.tmem, 0);
+    const int round_pairs = TC_TILES * TC_PAIRS, first_pair = it.tile * round_pairs, stride = it.tiles * round_pairs;
+    // (one round of pairs, unless the bound on a group's rows was too low; the barriers' phases go on counting)
 
-    for (int q0 = it.tile * TC_TILES * TC_PAIRS, round = 0; q0 < pairs; q0 += it.tiles * TC_TILES * TC_PAIRS, ++round) {
-        const int n_tiles = pairs - q0 > TC_PAIRS ? 2 : 1;
-        // queries: a pair a row of the tile, swizzled; pairs that are not there are zeros
-        for (int i = tid; i < n_tiles * TC_PAIRS * (D / 8); i += TC_THREADS) {
-            const int j = i / (D / 8), c = i % (D / 8), row = pair_row(a, it, q0 + j, share);
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (row >= 0)
-                v = *reinterpret_cast<const uint4*>((const bf16*)a.q + row * a.q_stride + (size_t)(kv_head * share + (q0 + j) % share) * D + c * 8);
-            *reinterpret_cast<uint4*>(q_tiles + (j / TC_PAIRS) * Z::TILE + (c / 8) * Z::ATOM + (j % TC_PAIRS) * 128 +
-                                      (((c % 8) ^ (j & 7)) * 16)) = v;
-        }
-        async_proxy_fence();
-        __syncthreads();
-
-        if (warp == TC_LOAD) {
-            int code = 0;
-            for (int j = 0; j < n_blocks; ++j) {
-                const int page = page_of(j), n = phase0 + j, stage = n % STAGES;
-                const int position = it.key0 + j * TC_KEYS + lane * box_rows;
-                // (no page: rows in front of the pool, which the copy fills with zeros)
-                const int y = page < 0 ? -box_rows : (page * a.n_kv_head + kv_head) * a.page_tokens + position % a.page_tokens;
+    if (warp < TC_SOFTMAX_WARPS) {
+        // warp: tile i, half h of the keys (and of the features), rows 32 * (warp % 4) .. of the tile
+        constexpr int HALF = TC_KEYS / 2, DH = D / 2;
+        const int i = warp / 8, h = (warp / 4) & 1, mine = tid & 127, pair_bar = 1 + i * 4 + (warp & 3);
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t o_at = lanes + TC_O_COL + i * D + h * DH;
+        // Whether any of the `threads` threads that meet at a barrier says so.  (All of them come to it, whatever they waited for in
+        // vain: a wait that ran out is told here, and all leave together.)
+        auto any_of = [&](int barrier, int threads, bool v) {
+            uint32_t any;
+            asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                         : "=r"(any) : "r"((uint32_t)v), "r"(barrier), "r"(threads) : "memory");
+            return any != 0u;
+        };
+        // the other half's number (the two warps of 32 pairs meet)
+        auto other_half = [&](float v) {
+            sync.meet[i][h][mine] = v;
+            asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
+            const float w = sync.meet[i][h ^ 1][mine];
+            asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
+            return w;
+        };
+        int n = 0, code = 0;                                            // blocks so far
+        bool holes = false;                                             // whether a page of the range is missing
+        for (int c = it.key0 / a.page_tokens + lane; c <= (it.key1 - 1) / a.page_tokens; c += 32) holes = holes || page_at(c) < 0;
+        holes = __any_sync(0xffffffffu, holes);
+        for (int q0 = first_pair, round = 0; q0 < pairs && code == 0; q0 += stride, ++round) {
+            const int j0 = q0 + i * TC_PAIRS;
+            if (j0 >= pairs) continue;                                  // no pairs for this tile
+            // queries: a pair a row of the tile, swizzled (pairs that are not there: zeros); a warp its 32 rows, all of a row's
+            // pieces by neighbouring lanes
+            const int row = pair_row(a, it, j0 + mine, share), head = kv_head * share + (j0 + mine) % share;
+            const long long q_at = row < 0 ? -1 : row * a.q_stride + (long long)head * D;
 #pragma unroll
-                for (int which = 0; which < 2; ++which) {
-                    uint64_t* const full = which ? &sync.v_full[stage] : &sync.k_full[stage];
-                    uint64_t* const free = which ? &sync.v_free[stage] : &sync.k_free[stage];
-                    if (n >= STAGES && !warp_wait(smem_u32(free), (n / STAGES - 1) & 1)) { code = 60; break; }
-                    if (lane == 0) mbar_expect_tx(smem_u32(full), Z::TILE);
-                    __syncwarp();
-                    if (lane < boxes)
-#pragma unroll
-                        for (int atom = 0; atom < ATOMS; ++atom)
-                            tma_load_2d(smem_u32((which ? v_tiles : k_tiles) + stage * Z::TILE + atom * Z::ATOM + lane * box_rows * 128),
-                                        which ? &map_v : &map_k, smem_u32(full), atom * 64, y);
-                    __syncwarp();
-                }
-                if (code) break;
+            for (int e = h * (D / 16); e < (h + 1) * (D / 16); ++e) {
+                constexpr int ROWS = 256 / D;                           // rows at once: 32 lanes of 8 features
+                const int r = e * ROWS + lane / (D / 8), c = lane % (D / 8);
+                const long long from = __shfl_sync(0xffffffffu, q_at, r);
+                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                if (from >= 0) v = *reinterpret_cast<const uint4*>((const bf16*)a.q + from + c * 8);
+                *reinterpret_cast<uint4*>(q_tiles + i * Z::Q_TILE + (c / 8) * Z::Q_ATOM + ((warp & 3) * 32 + r) * 128 + (((c % 8) ^ (r & 7)) * 16)) = v;
             }
-            if (code) {
-                if (lane == 0) { atomicExch(status, code); *(volatile uint32_t*)&sync.failed = 1; }
-                good = false;
-            }
-        } else if (warp == TC_ISSUE) {
-            auto scores = [&](int j, int i) {                           // S_i(j) = Q_i K(j)^T
-                const int n = phase0 + j, stage = n % STAGES;
-                if (i == 0 && !warp_wait(smem_u32(&sync.k_full[stage]), (n / STAGES) & 1)) return false;
+            async_proxy_fence();
+            tc_fence_before();
+            mbar_arrive(smem_u32(&sync.q_ready[i]));
+            float ref = -INFINITY, total = 0.f;
+            for (int b = 0; b < n_blocks; ++b, ++n) {
+                const int last = it.key1 - it.key0 - b * TC_KEYS;       // keys of this block
+                const uint32_t buffer = lanes + (i * 2 + (n & 1)) * TC_KEYS, s_at = buffer + h * HALF;      // (P of a half: in front)
+                if (code == 0 && !warp_wait(smem_u32(&sync.s_full[i][n & 1]), (n >> 1) & 1)) code = 64;
                 tc_fence_after();
-                if (elect_one()) {
-                    constexpr uint32_t idesc = instr_desc_bf16(TC_PAIRS, TC_KEYS, false);
-                    const uint64_t dq = smem_desc_sw128(smem_u32(q_tiles + i * Z::TILE)), dk = smem_desc_sw128(smem_u32(k_tiles + stage * Z::TILE));
+                uint32_t s[HALF];
 #pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        const uint64_t step = (uint64_t)((k / 4 * Z::ATOM + k % 4 * 32) >> 4);
-                        umma_bf16(tmem + i * TC_KEYS, dq + step, dk + step, idesc, k ? 1u : 0u);
-                    }
-                    umma_commit(smem_u32(&sync.s_full[i]));
-                    if (i == n_tiles - 1) umma_commit(smem_u32(&sync.k_free[stage]));
+                for (int c = 0; c < HALF / 32; ++c) tmem_load_32(s_at + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
+                tmem_wait_ld();
+                if (last < TC_KEYS || holes) {
+                    // keys behind the range's end, and those whose page is missing
+                    const int position = it.key0 + b * TC_KEYS + lane * box_rows;
+                    const uint32_t there = __ballot_sync(0xffffffffu, lane < boxes && position < it.key1 && page_at(position / a.page_tokens) >= 0);
+#pragma unroll
+                    for (int c = 0; c < HALF; ++c)
+                        if (h * HALF + c >= last || !((there >> ((h * HALF + c) >> box_shift)) & 1u)) s[c] = 0xff800000u;
                 }
-                __syncwarp();
-                return true;
-            };
-            int code = 0;
-            for (int i = 0; i < n_tiles && code == 0; ++i)
-                if (!scores(0, i)) code = 61;
-            for (int j = 0; j < n_blocks && code == 0; ++j) {
-                const int n = phase0 + j, stage = n % STAGES;
-                for (int i = 0; i < n_tiles && code == 0; ++i) {
-                    if (!warp_wait(smem_u32(&sync.p_ready[i]), n & 1)) { code = 62; break; }
-                    if (i == 0 && !warp_wait(smem_u32(&sync.v_full[stage]), (n / STAGES) & 1)) { code = 63; break; }
-                    tc_fence_after();
-                    if (elect_one()) {
-                        constexpr uint32_t idesc = instr_desc_bf16(TC_PAIRS, 64, true);
+                bool move = ref == -INFINITY;
+                float sum = 0.f;
+#pragma unroll 1
+                for (int pass = 0; pass < 3; ++pass) {
+                    if (pass > 0 || __any_sync(0xffffffffu, move)) {        // (the two threads of a pair agree on ref)
+                        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, corr = 1.f;
 #pragma unroll
-                        for (int atom = 0; atom < ATOMS; ++atom)
-#pragma unroll
-                            for (int k = 0; k < TC_KEYS / 16; ++k)
-                                umma_bf16_ts(tmem + TC_O_COL + i * D + atom * 64, tmem + i * TC_KEYS + k * 8,
-                                             smem_desc_sw128(smem_u32(v_tiles + stage * Z::TILE + atom * Z::ATOM + k * (16 * 128))), idesc,
-                                             (j | k) ? 1u : 0u);
-                        if (i == n_tiles - 1) {
-                            umma_commit(smem_u32(&sync.v_free[stage]));
-                            if (j == n_blocks - 1) umma_commit(smem_u32(&sync.done));
-                        }
-                    }
-                    __syncwarp();
-                    // (in order behind the product that reads P in S's place)
-                    if (j + 1 < n_blocks && !scores(j + 1, i)) code = 61;
-                }
-            }
-            if (code) {
-                if (lane == 0) { atomicExch(status, code); *(volatile uint32_t*)&sync.failed = 1; }
-                good = false;
-            }
-        } else {
-            const int i = warp / 4, j = q0 + i * TC_PAIRS + (tid & 127);
-            if (i < n_tiles) {
-                const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), s_at = lanes + i * TC_KEYS, o_at = lanes + TC_O_COL + i * D;
-                float ref = -INFINITY, total = 0.f;
-                int page = page_of(0);
-                for (int b = 0; b < n_blocks; ++b) {
-                    const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
-                    if (b + 1 < n_blocks) page = page_of(b + 1);
-                    const int n = phase0 + b, stage = n % STAGES, last = it.key1 - it.key0 - b * TC_KEYS;     // keys of this block
-                    if (!warp_wait(smem_u32(&sync.s_full[i]), n & 1)) { good = false; atomicExch(status, 64); break; }
-                    tc_fence_after();
-                    uint32_t s[TC_KEYS];
-#pragma unroll
-                    for (int c = 0; c < TC_KEYS / 32; ++c) tmem_load_32(s_at + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
-                    tmem_wait_ld();
-                    if (last < TC_KEYS || there != (uint32_t)((1ull << boxes) - 1)) {
-#pragma unroll
-                        for (int c = 0; c < TC_KEYS; ++c)
-                            if (c >= last || !((there >> (c >> box_shift)) & 1u)) s[c] = 0xff800000u;
-                    }
-                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int c = 0; c < TC_KEYS; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(s[c]));
-                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2e;
-                    const bool high = top > ref + TC_SLACK;             // (also the first block that has a key at all)
-                    if (__any_sync(0xffffffffu, high)) {
-                        float corr = 1.f;
-                        if (high) {
-                            corr = ref == -INFINITY ? 0.f : exp2f(ref - top);
+                        for (int c = 0; c < HALF; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(s[c]));
+                        float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2e;
+                        top = fmaxf(top, other_half(top));
+                        move = other_half(move ? 1.f : 0.f) != 0.f || move;
+                        if (move) {
+                            corr = ref == -INFINITY ? 1.f : exp2f(ref - top);      // (nothing was summed before the first)
                             ref = top;
                         }
                         total *= corr;
-                        if (b > 0) {                                    // (the products before this block's scores are over)
+                        if (b > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
+                            // once the block before is in the average (that the one before it is, these scores have shown)
+                            if (!warp_wait(smem_u32(&sync.pv_done[i]), (n - 1) & 1)) code = 68;
+                            tc_fence_after();
 #pragma unroll
-                            for (int c = 0; c < D / 16; ++c) {
-                                uint32_t r[16];
-                                tmem_load_16(o_at + c * 16, r);
+                            for (int c = 0; c < DH / 8; ++c) {
+                                uint32_t r[8];
+                                tmem_load_8(o_at + c * 8, r);
                                 tmem_wait_ld();
 #pragma unroll
-                                for (int k = 0; k < 16; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * corr);
-                                tmem_store_16(o_at + c * 16, r);
+                                for (int k = 0; k < 8; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * corr);
+                                tmem_store_8(o_at + c * 8, r);
                             }
                         }
                     }
+                    // P in the scores' place, and the row's sum
                     const float shift = ref == -INFINITY ? 0.f : ref;
                     float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int h = 0; h < 4; ++h) {
-                        uint32_t p[16];
+                    for (int w = 0; w < HALF / 16; ++w) {
+                        uint32_t p[8];
 #pragma unroll
-                        for (int c = 0; c < 16; ++c) {
-                            const float e0 = exp2_approx(fmaf(__uint_as_float(s[h * 32 + 2 * c]), a.scale_log2e, -shift));
-                            const float e1 = exp2_approx(fmaf(__uint_as_float(s[h * 32 + 2 * c + 1]), a.scale_log2e, -shift));
+                        for (int c = 0; c < 8; ++c) {
+                            const float e0 = exp2_approx(fmaf(__uint_as_float(s[w * 16 + 2 * c]), a.scale_log2e, -shift));
+                            const float e1 = exp2_approx(fmaf(__uint_as_float(s[w * 16 + 2 * c + 1]), a.scale_log2e, -shift));
                             part[c & 3] += e0 + e1;
                             p[c] = pack_bf16(e0, e1);
                         }
-                        tmem_store_16(s_at + h * 16, p);
+                        tmem_store_8(s_at + w * 8, p);
                     }
-                    total += (part[0] + part[1]) + (part[2] + part[3]);
-                    // value rows behind the range's last key hold whatever is in the page: 0 times that has to be 0
-                    if (last < TC_KEYS && i == 0) {
-                        if (!warp_wait(smem_u32(&sync.v_full[stage]), (n / STAGES) & 1)) { good = false; atomicExch(status, 65); break; }
-                        if (tid >= last)
+                    sum = (part[0] + part[1]) + (part[2] + part[3]);
+                    move = !(sum <= TC_LIMIT);
+                    if (!any_of(pair_bar, 64, move || code != 0)) break;
+                    if (other_half(code != 0 ? 1.f : 0.f) != 0.f && code == 0) code = 71;       // the other warp waited in vain
+                }
+                if (code != 0) break;                                   // (the same in both warps)
+                total += sum;
+                // value rows behind the range's last key hold whatever is in the page: 0 times that has to be 0 (both tiles write
+                // the same zeros: neither waits for the other)
+                if (last < TC_KEYS && h == 0) {
+                    const int stage = n % STAGES;
+                    if (!warp_wait(smem_u32(&sync.v_full[stage]), (n / STAGES) & 1)) code = 65;
+                    if (mine >= last && mine < TC_KEYS)
+#pragma unroll
+                        for (int atom = 0; atom < ATOMS; ++atom)
+#pragma unroll
+                            for (int c = 0; c < 8; ++c)
+                                *reinterpret_cast<uint4*>(v_tiles + stage * Z::TILE + atom * Z::ATOM + mine * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    async_proxy_fence();
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(smem_u32(&sync.p_ready[i][n & 1]));
+            }
+            // (a barrier of its own: pv_done may be two phases behind here, and their parities are alike)
+            if (code == 0 && !warp_wait(smem_u32(&sync.round_done[i]), round & 1)) code = 66;
+            tc_fence_after();
+            // the averages: 16 features at a time by way of the tile's queries' place, so that neighbouring lanes write
+            // neighbouring numbers
+            const bool write = row >= 0 && code == 0 && *(volatile uint32_t*)&sync.failed == 0;
+            const long long at = write ? ((long long)row * a.n_head + head) * (a.shared_slots + a.own_slots) + it.slot : -1;
+            float4* const scratch = reinterpret_cast<float4*>(q_tiles + i * Z::Q_TILE + (warp & 7) * 2048);
+#pragma unroll
+            for (int c = 0; c < DH / 16; ++c) {
+                uint32_t r[16];
+                tmem_load_16(o_at + c * 16, r);
+                tmem_wait_ld();
+                __syncwarp();
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    scratch[lane * 4 + (k ^ ((lane >> 1) & 3))] = make_float4(__uint_as_float(r[4 * k]), __uint_as_float(r[4 * k + 1]),
+                                                                              __uint_as_float(r[4 * k + 2]), __uint_as_float(r[4 * k + 3]));
+                __syncwarp();
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int from = k * 8 + lane / 4, piece = lane & 3;
+                    const long long to = __shfl_sync(0xffffffffu, at, from);
+                    if (to >= 0)
+                        *reinterpret_cast<float4*>(a.part_out + to * D + h * DH + c * 16 + piece * 4) = scratch[from * 4 + (piece ^ ((from >> 1) & 3))];
+                }
+            }
+            total += other_half(total);
+            if (write && h == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(ref, total);
+            // (the queries' place is scratch no more)
+            if (any_of(9 + i, 256, code != 0) && code == 0) code = 69;
+        }
+        if (code) {
+            atomicExch(status, code);
+            *(volatile uint32_t*)&sync.failed = 1;
+        }
+    } else {
+        int code = 0;
+        if (warp == TC_LOAD) {
+            int n = 0;
+            for (int q0 = first_pair; q0 < pairs && code == 0; q0 += stride) {
+                // box `lane` of the blocks; its page is looked up a block ahead (pages smaller than a block: a box each; larger
+                // ones begin at a block)
+                int position = it.key0 + lane * box_rows, column = position / a.page_tokens, offset = position - column * a.page_tokens;
+                auto look = [&]() { return lane < boxes && position < it.key1 && column < a.max_pages ? it.table[column] : -1; };
+                int page = look();
+                for (int b = 0; b < n_blocks && code == 0; ++b, ++n) {
+                    const int stage = n % STAGES;
+                    if (page >= a.num_pages) page = -1;
+                    if (page >= 0 && !MG_GUARDED(attention_shared, MG_GUARD_PAGE, page, a.num_pages)) page = -1;
+                    // (no page: rows in front of the pool, which the copy fills with zeros)
+                    const int y = page < 0 ? -box_rows : (page * a.n_kv_head + kv_head) * a.page_tokens + offset;
+                    position += TC_KEYS;
+                    if (a.page_tokens < TC_KEYS) column += boxes;
+                    else if ((offset += TC_KEYS) >= a.page_tokens) { offset = 0; ++column; }
+                    page = look();
+#pragma unroll
+                    for (int which = 0; which < 2; ++which) {
+                        uint64_t* const full = which ? &sync.v_full[stage] : &sync.k_full[stage];
+                        uint64_t* const free = which ? &sync.v_free[stage] : &sync.k_free[stage];
+                        if (n >= STAGES && !warp_wait(smem_u32(free), (n / STAGES - 1) & 1)) { code = 60; break; }
+                        if (lane == 0) mbar_expect_tx(smem_u32(full), Z::TILE);
+                        __syncwarp();
+                        if (lane < boxes)
 #pragma unroll
                             for (int atom = 0; atom < ATOMS; ++atom)
-#pragma unroll
-                                for (int c = 0; c < 8; ++c)
-                                    *reinterpret_cast<uint4*>(v_tiles + stage * Z::TILE + atom * Z::ATOM + tid * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
-                        async_proxy_fence();
+                                tma_load_2d(smem_u32((which ? v_tiles : k_tiles) + stage * Z::TILE + atom * Z::ATOM + lane * box_rows * 128),
+                                            which ? &map_v : &map_k, smem_u32(full), atom * 64, y);
+                        __syncwarp();
                     }
-                    tmem_wait_st();
-                    tc_fence_before();
-                    mbar_arrive(smem_u32(&sync.p_ready[i]));
                 }
-                if (good && !warp_wait(smem_u32(&sync.done), round & 1)) { good = false; atomicExch(status, 66); }
-                tc_fence_after();
-                const int row = pair_row(a, it, j, share);
-                const bool failed = !good || *(volatile uint32_t*)&sync.failed != 0;
-                const size_t at = ((size_t)max(row, 0) * a.n_head + kv_head * share + j % share) * (a.shared_slots + a.own_slots) + it.slot;
-                float4* const dst = reinterpret_cast<float4*>(a.part_out + at * D);
+            }
+        } else {
+            // a warp a tile: each waits for its own softmax and products, so that the other's fill the time
+            const int i = warp - TC_ISSUE;
+            int n = 0;
+            for (int q0 = first_pair, round = 0; q0 < pairs && code == 0; q0 += stride, ++round) {
+                const bool active = q0 + i * TC_PAIRS < pairs;
+                auto scores = [&](int m) {                              // S of block m = Q K^T
+                    const int stage = m % STAGES;
+                    if (!warp_wait(smem_u32(&sync.k_full[stage]), (m / STAGES) & 1)) return false;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        constexpr uint32_t idesc = instr_desc_bf16(TC_PAIRS, TC_KEYS, false);
+                        const uint64_t dq = smem_desc_sw128(smem_u32(q_tiles + i * Z::Q_TILE)), dk = smem_desc_sw128(smem_u32(k_tiles + stage * Z::TILE));
 #pragma unroll
-                for (int c = 0; c < D / 32; ++c) {
-                    uint32_t r[32];
-                    tmem_load_32(o_at + c * 32, r);
-                    tmem_wait_ld();
-                    if (row >= 0 && !failed)
-#pragma unroll
-                        for (int k = 0; k < 8; ++k)
-                            dst[c * 8 + k] = make_float4(__uint_as_float(r[4 * k]), __uint_as_float(r[4 * k + 1]), __uint_as_float(r[4 * k + 2]),
-                                                         __uint_as_float(r[4 * k + 3]));
+                        for (int k = 0; k < D / 16; ++k)
+                            umma_bf16(tmem + (i * 2 + (m & 1)) * TC_KEYS, dq + (uint64_t)((k / 4 * Z::Q_ATOM + k % 4 * 32) >> 4),
+                                      dk + (uint64_t)((k / 4 * Z::ATOM + k % 4 * 32) >> 4), idesc, k ? 1u : 0u);
+                        umma_commit(smem_u32(&sync.s_full[i][m & 1]));
+                        umma_commit(smem_u32(&sync.k_free[stage]));
+                    }
+                    __syncwarp();
+                    return true;
+                };
+                if (!active) {                                          // no pairs for this tile: it gives the blocks back unread
+                    for (int b = 0; b < n_blocks && code == 0; ++b, ++n) {
+                        const int stage = n % STAGES;
+                        if (!warp_wait(smem_u32(&sync.k_full[stage]), (n / STAGES) & 1) || !warp_wait(smem_u32(&sync.v_full[stage]), (n / STAGES) & 1)) {
+                            code = 61;
+                        } else if (lane == 0) {
+                            mbar_arrive(smem_u32(&sync.k_free[stage]));
+                            mbar_arrive(smem_u32(&sync.v_free[stage]));
+                        }
+                    }
+                    continue;
                 }
-                if (row >= 0 && !failed) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(ref, total);
+                if (!warp_wait(smem_u32(&sync.q_ready[i]), round & 1)) { code = 67; break; }
+                if (!scores(n) || (n_blocks > 1 && !scores(n + 1))) code = 61;
+                for (int b = 0; b < n_blocks && code == 0; ++b, ++n) {
+                    const int stage = n % STAGES;
+                    if (!warp_wait(smem_u32(&sync.p_ready[i][n & 1]), (n >> 1) & 1)) { code = 62; break; }
+                    if (!warp_wait(smem_u32(&sync.v_full[stage]), (n / STAGES) & 1)) { code = 63; break; }
+                    tc_fence_after();
+                    if (elect_one()) {
+                        constexpr uint32_t idesc = instr_desc_bf16(TC_PAIRS, D, true);
+                        // (values: atoms of 64 features, the second an atom's bytes behind the first)
+                        const uint64_t dv = smem_desc_sw128(smem_u32(v_tiles + stage * Z::TILE)) + ((uint64_t)((Z::ATOM >> 4) - 1) << 16);
+#pragma unroll
+                        for (int k = 0; k < TC_KEYS / 16; ++k)
+                            umma_bf16_ts(tmem + TC_O_COL + i * D, tmem + (i * 2 + (n & 1)) * TC_KEYS + (k / 2) * (TC_KEYS / 2) + (k % 2) * 8, dv + (uint64_t)(k * (16 * 128) >> 4), idesc,
+                                         (b | k) ? 1u : 0u);
+                        umma_commit(smem_u32(&sync.pv_done[i]));
+                        umma_commit(smem_u32(&sync.v_free[stage]));
+                        if (b == n_blocks - 1) umma_commit(smem_u32(&sync.round_done[i]));
+                    }
+                    __syncwarp();
+                    // the scores of the block after the next, in the place of the P that has just gone into the average (only the wait
+                    // orders the two)
+                    if (b + 2 < n_blocks && (!warp_wait(smem_u32(&sync.pv_done[i]), n & 1) || !scores(n + 2))) code = 61;
+                }
             }
         }
-        tc_fence_before();
-        good = __syncthreads_and(good) && *(volatile uint32_t*)&sync.failed == 0;
-        tc_fence_after();
-        if (!good) break;
-        phase0 += n_blocks;
+        if (code && lane == 0) {
+            atomicExch(status, code);
+            *(volatile uint32_t*)&sync.failed = 1;
+        }
     }
-    if (!good && tid == 0)
+    tc_fence_before();
+    __syncthreads();
+    if (*(volatile uint32_t*)&sync.failed != 0 && tid == 0)
         for (int i = 0; i < 2000; ++i) __nanosleep(1000);               // let copies in flight land
     __syncthreads();
     if (warp == TC_ISSUE) tmem_dealloc(tmem, TC_COLS);
 }
 
 // ---- the ranges of a (row, head) joined: a warp each ------------------------------------------------------------------
-template <typename T>
+// J: features a lane takes (lane, lane + 32, ..).  Eight ranges are asked for at once.
+template <typename T, int J>
 __global__ void __launch_bounds__(128) attention_shared_join_kernel(SharedArgs a) {
-    __shared__ int hold;
     const int row = blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const int p = a.positions[row];
-    int behind = group_tokens(a, row, &hold);
-    if (behind > p + 1) behind = 0;
     if (head >= a.n_head) return;
-    T* out = (T*)a.out + ((size_t)row * a.n_head + head) * a.D;
+    const int p = a.positions[row];
+    T* const out = (T*)a.out + ((size_t)row * a.n_head + head) * a.D;
+    pdl_wait();
+    pdl_trigger();
+    const int behind = a.behind[row], own = p + 1 - behind;
     if (p < 0) {                                          // padding of a fixed-size batch
         for (int d = lane; d < a.D; d += 32) out[d] = from_float<T>(0.f);
         return;
     }
-    const int shared_step = range_keys(behind, a.shared_slots, a.shared_least), own = p + 1 - behind;
-    const int own_step = range_keys(own, a.own_slots, OWN_LEAST);
+    const int shared_step = range_keys(behind, a.shared_slots, a.shared_least), own_step = range_keys(own, a.own_slots, OWN_LEAST);
     const int n_shared = (behind + shared_step - 1) / shared_step, n_all = n_shared + (own + own_step - 1) / own_step;
     const size_t base = ((size_t)row * a.n_head + head) * (a.shared_slots + a.own_slots);
     const int skip = a.shared_slots - n_shared;           // slots of shared ranges that this length does not have
-    float top = -INFINITY;
-    for (int i = lane; i < n_all; i += 32) top = fmaxf(top, a.part_ml[(base + i + (i < n_shared ? 0 : skip)) * 2]);
-    top = warp_max(top);
-    float acc[8], total = 0.f;
+    // averages relative to the largest maximum so far
+    float top = -INFINITY, total = 0.f, acc[J];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = 0.f;
-    for (int i = 0; i < n_all; ++i) {
-        const size_t at = base + i + (i < n_shared ? 0 : skip);
-        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
-        const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
-        total = fmaf(w, ml.y, total);
+    for (int j = 0; j < J; ++j) acc[j] = 0.f;
+    for (int i0 = 0; i0 < n_all; i0 += 8) {
+        float x[8][J];
+        float2 ml[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (lane + 32 * j < a.D) acc[j] = fmaf(w, a.part_out[at * a.D + lane + 32 * j], acc[j]);
+        for (int u = 0; u < 8; ++u) {
+            const bool in = i0 + u < n_all;
+            const size_t at = base + i0 + u + (i0 + u < n_shared ? 0 : skip);
+            ml[u] = in ? *reinterpret_cast<const float2*>(a.part_ml + at * 2) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int j = 0; j < J; ++j) x[u][j] = in && lane + 32 * j < a.D ? a.part_out[at * a.D + lane + 32 * j] : 0.f;
+        }
+        float high = top;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) high = fmaxf(high, ml[u].x);
+        const float corr = top == -INFINITY ? 0.f : exp2f(top - high);
+        top = high;
+        total *= corr;
+#pragma unroll
+        for (int j = 0; j < J; ++j) acc[j] *= corr;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {                     // ranges in order
+            if (ml[u].x == -INFINITY) continue;
+            const float w = exp2f(ml[u].x - top);
+            total = fmaf(w, ml[u].y, total);
+#pragma unroll
+            for (int j = 0; j < J; ++j) acc[j] = fmaf(w, x[u][j], acc[j]);
+        }
     }
-    const float inv = total > 0.f ? 1.0f / total : 0.f;   // (no key has a page: zeros)
+    const float inv = total != 0.f ? 1.0f / total : 0.f;  // (no key has a page: zeros)
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int j = 0; j < J; ++j)
         if (lane + 32 * j < a.D) out[lane + 32 * j] = from_float<T>(acc[j] * inv);
+}
+
+// A kernel that may start while the one in front of it, which is this operator's own, still runs.
+template <typename... KArgs>
+int launch_behind(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t s, const SharedArgs& a) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+    if (e != cudaSuccess) return mg_set_error(MG_ERR_CUDA, "attention (shared): %s", cudaGetErrorString(e));
+    MG_CHECK_LAUNCH("attention (shared)");
+    return MG_OK;
 }
 
 template <typename T>
 int launch_join(const SharedArgs& a, cudaStream_t s) {
-    attention_shared_join_kernel<T><<<dim3(a.n, ceil_div(a.n_head, 4)), 128, 0, s>>>(a);
-    MG_CHECK_LAUNCH("attention (shared, join)");
-    return MG_OK;
+    const auto kernel = a.D <= 32 ? attention_shared_join_kernel<T, 1> : a.D <= 64 ? attention_shared_join_kernel<T, 2>
+                        : a.D <= 128 ? attention_shared_join_kernel<T, 4> : attention_shared_join_kernel<T, 8>;
+    return launch_behind(kernel, dim3(a.n, ceil_div(a.n_head, 4)), 128, 0, s, a);
 }
 
 template <typename... KArgs>
@@ -857,7 +1006,10 @@ int launch_ranges(void (*kernel)(KArgs...), int threads, size_t smem, const Shar
     const cudaError_t e = mg_raise_shared(kernel, smem);
     if (e != cudaSuccess) return mg_set_error(MG_ERR_CUDA, "attention (shared): cannot raise shared memory: %s", cudaGetErrorString(e));
     const long long items = (long long)a.n_groups * a.row_tiles * a.shared_slots + (long long)a.n * a.own_slots - a.first_item;
-    kernel<<<dim3((unsigned)items, a.n_kv_head), threads, smem, s>>>(a);
+    const dim3 grid((unsigned)items, a.n_kv_head);
+    if (a.first_item > 0) return launch_behind(kernel, grid, threads, smem, s, a);
+    const cudaError_t le = mg_launch(kernel, grid, dim3(threads), smem, s, true, a);
+    if (le != cudaSuccess) return mg_set_error(MG_ERR_CUDA, "attention (shared): %s", cudaGetErrorString(le));
     MG_CHECK_LAUNCH("attention (shared)");
     return MG_OK;
 }
@@ -871,13 +1023,14 @@ int launch_tc(const SharedArgs& a, int* status, cudaStream_t s) {
     if (rc != MG_OK) return rc;
     const cudaError_t e = mg_raise_shared(attention_shared_tc_kernel<D>, TcSizes<D>::SMEM);
     if (e != cudaSuccess) return mg_set_error(MG_ERR_CUDA, "attention (shared): cannot raise shared memory: %s", cudaGetErrorString(e));
-    attention_shared_tc_kernel<D><<<dim3((unsigned)(a.n_groups * a.row_tiles * a.shared_slots), a.n_kv_head), TC_THREADS, TcSizes<D>::SMEM, s>>>(
-        a, map_k, map_v, box_rows, status);
+    const cudaError_t le = mg_launch(attention_shared_tc_kernel<D>, dim3((unsigned)(a.n_groups * a.row_tiles * a.shared_slots), a.n_kv_head),
+                                     dim3(TC_THREADS), TcSizes<D>::SMEM, s, true, a, map_k, map_v, box_rows, status);
+    if (le != cudaSuccess) return mg_set_error(MG_ERR_CUDA, "attention (shared, tcgen05): %s", cudaGetErrorString(le));
     MG_CHECK_LAUNCH("attention (shared, tcgen05)");
     return MG_OK;
 }
 
-constexpr int TC_LEAST_PAIRS = 64;
+constexpr int TC_LEAST_PAIRS = 64, TC_CTA_KEYS = 1000;
 
 template <int DP>
 int launch_mma(const SharedArgs& a, int pair_tiles, cudaStream_t s) {
@@ -919,7 +1072,15 @@ Cut cut(int n_groups, int max_rows, int max_tokens, int max_behind, int n, int n
     const int most_shared = ceil_div(max_tokens > 0 ? max_tokens : 1, c.shared_least), most_own = ceil_div(max_behind, OWN_LEAST);
     const long long want = 148 * 4;
     long long x = shared_ctas > 0 ? (want + shared_ctas - 1) / shared_ctas : 1;
-    if (c.tc) x = 148 / shared_ctas;                       // one CTA an SM
+    if (c.tc) {
+        // one CTA an SM: the number of ranges whose rounds of CTAs take the fewest keys, what a CTA costs besides its keys
+        // counted as TC_CTA_KEYS of them
+        double best = 0.0;
+        for (int r = 1; r <= most_shared && r <= 64; ++r) {
+            const double cost = (double)((shared_ctas * r + 147) / 148) * ((double)max_tokens / r + TC_CTA_KEYS);
+            if (r == 1 || cost < best) { best = cost; x = r; }
+        }
+    }
     const long long y = (want + own_ctas - 1) / own_ctas;
     c.shared_slots = (int)(x < 1 ? 1 : x > most_shared ? most_shared : x);
     c.own_slots = (int)(y < 1 ? 1 : y > most_own ? most_own : y);
@@ -934,7 +1095,7 @@ MG_API long long mg_attention_shared_scratch_floats(int n_groups, int max_rows, 
     if (n_groups < 0 || max_rows <= 0 || n <= 0 || n_head <= 0 || n_kv_head <= 0 || n_head % n_kv_head != 0 || max_behind <= 0 || page_tokens <= 0) return 0;
     const Cut c = cut(n_groups, max_rows, max_tokens, max_behind, n, n_head, n_kv_head, head_dim, page_tokens, is_bf16 != 0);
     const size_t slots = (size_t)n * n_head * (c.shared_slots + c.own_slots);
-    return (long long)(sums_at(slots, head_dim) + 2 * slots);
+    return (long long)(sums_at(slots, head_dim) + 2 * slots + n);
 }
 
 MG_API int mg_attention_shared_launches(int n_groups, int max_rows, int max_tokens, int max_behind, int n, int n_head, int n_kv_head,
@@ -979,6 +1140,7 @@ MG_API int mg_attention_shared(const void* q, long long q_stride, const void* k_
     const size_t slots = (size_t)n * n_head * (c.shared_slots + c.own_slots);
     a.part_out = scratch;
     a.part_ml = scratch + sums_at(slots, head_dim);
+    a.behind = (int*)(a.part_ml + 2 * slots);
     const long long items = (long long)n_groups * c.row_tiles * c.shared_slots + (long long)n * c.own_slots;
     MG_REQUIRE(items < (1ll << 31), "attention (shared): too many rows");
     cudaStream_t s = (cudaStream_t)stream;
