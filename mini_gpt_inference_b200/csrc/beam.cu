@@ -6,12 +6,14 @@
 // tokens of the continuation.  The B best go on.  Equal ranks go to the lower row; within a row the order is that of the
 // logits, equal ones by the lower id, so a row's B largest logits are all that a row can contribute, whatever L_b is:
 //
-//   rows kernel    one pass over the logits: every warp keeps the running maximum and sum of its piece (for L_b) and the B
-//                  best (logit, id) pairs as a sorted list, one 64-bit key a lane (the logit's bits in an order that
-//                  unsigned numbers have, then the id from above: all keys differ, so ties need no care).  A CTA's eight
-//                  lists become one by bitonic merges.
-//   choice kernel  one CTA a group: the rows' lists and sums joined, values in 64 bits, and B times the best of the
-//                  rows' first candidates.
+//   rows kernel    one pass over the logits: every lane of a CTA keeps the maximum and sum of its own (for L_b).  The B best
+//                  logits of the CTA's piece lie in the B lanes with the largest maxima; those lanes' logits are looked at again.
+//                  (logit, id) pairs are 64-bit keys, the logit's bits in an order that unsigned numbers have, then the id
+//                  from above: all keys differ, so ties need no care.  Lists are sorted over a warp's lanes and joined by
+//                  bitonic merges.  (Every warp keeping the B best of its piece as it reads: 768 instructions for 512 logits
+//                  of 50,257 and B = 16, and bound by them: 85 us for 64 x 16 rows.)
+//   choice kernel  one CTA a group: the rows' lists and sums joined, values in 64 bits, and a thread a candidate that counts
+//                  those in front of it.
 //
 // A beam that goes on stays in its row: its best continuation takes the row, its others take, in order of rank, the rows
 // whose beams do not go on.  So only those rows' caches change hands, a row that is read is never written (reorder needs
@@ -44,6 +46,8 @@ __device__ __forceinline__ u64 order_of(double x) {
     return b ^ ((b >> 63) ? ~0ull : 1ull << 63);
 }
 
+__device__ __forceinline__ u64 key_of(float x, int id) { return ((u64)order_of(x) << 32) | (uint32_t)~(uint32_t)id; }
+
 __device__ __forceinline__ u64 max64(u64 a, u64 b) { return a > b ? a : b; }
 __device__ __forceinline__ u64 min64(u64 a, u64 b) { return a < b ? a : b; }
 
@@ -58,94 +62,21 @@ __device__ __forceinline__ u64 merge_lists(u64 a, u64 b, int lane) {
     return c;
 }
 
-// The lanes' numbers sorted downwards.
-__device__ __forceinline__ uint32_t sort_lanes(uint32_t v, int lane) {
+// The lanes' keys sorted downwards.
+__device__ __forceinline__ u64 sort_lanes(u64 v, int lane) {
 #pragma unroll
     for (int k = 2; k <= 32; k <<= 1)
 #pragma unroll
         for (int o = k >> 1; o > 0; o >>= 1) {
-            const uint32_t other = __shfl_xor_sync(0xffffffffu, v, o);
-            const bool larger = ((lane & k) == 0) == ((lane & o) == 0);
-            v = larger ? max(v, other) : min(v, other);
+            const u64 other = __shfl_xor_sync(0xffffffffu, v, o);
+            v = ((lane & k) == 0) == ((lane & o) == 0) ? max64(v, other) : min64(v, other);
         }
     return v;
 }
 
-__global__ void __launch_bounds__(ROW_THREADS)
-beam_rows_kernel(const float* __restrict__ logits, const int* __restrict__ ended, u64* __restrict__ lists, float* __restrict__ sums,
-                 int vocab, int limit, int beams, int chunk) {
-    __shared__ u64 meet[ROW_WARPS][32];
-    __shared__ float meet_max[ROW_WARPS], meet_sum[ROW_WARPS];
-    const int row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    pdl_trigger();
-    pdl_wait();
-    if (ended != nullptr && ended[row] != 0) return;       // its one candidate is itself
-    const float* const base = logits + (size_t)row * vocab;
-    // ids are counted from the 16-byte boundary at or in front of the row's first logit
-    const int lead = (int)(((uintptr_t)base >> 2) & 3);
-    const int begin = (blockIdx.x * ROW_WARPS + warp) * chunk, end = min(limit + lead, begin + chunk);
-    u64 list = 0, least = 0;                                // lane i: the warp's i-th best; its beams-th best
-    float top = -INFINITY, sum = 0.f;
-    const float log2e = 1.4426950408889634f;
-    for (int b0 = begin; b0 < end; b0 += BATCH) {
-        float x[16];
-        uint32_t o[16];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int j = b0 + q * 128 + lane * 4;
-            if (j >= lead && j + 4 <= end) {
-                const float4 v = *reinterpret_cast<const float4*>(base + (j - lead));
-                x[4 * q] = v.x; x[4 * q + 1] = v.y; x[4 * q + 2] = v.z; x[4 * q + 3] = v.w;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[4 * q + i] = (j + i >= lead && j + i < end) ? base[j + i - lead] : -INFINITY;
-            }
-        }
-        float high = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            if (!(x[e] == x[e])) x[e] = -INFINITY;
-            high = fmaxf(high, x[e]);
-        }
-        // the sum, relative to the largest so far
-        if (high > top) {
-            sum *= exp2f((top - high) * log2e);
-            top = high;
-        }
-        const float shift = top == -INFINITY ? 0.f : top;
-        float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int e = 0; e < 16; ++e) part[e & 3] += exp2_approx((x[e] - shift) * log2e);
-        sum += (part[0] + part[1]) + (part[2] + part[3]);
-        // candidates: nothing at all in most batches behind the first
-        uint32_t coarse = (uint32_t)(least >> 32);
-        const uint32_t mine = order_of(high);
-        // the first batch: `beams` lanes have a logit of at least the beams-th largest of the lanes' largest ones
-        if (least == 0) coarse = __shfl_sync(0xffffffffu, sort_lanes(mine, lane), beams - 1);
-        if (__any_sync(0xffffffffu, mine >= coarse)) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int j = b0 + (e >> 2) * 128 + lane * 4 + (e & 3);
-                o[e] = (j >= lead && j < end) ? order_of(x[e]) : 0u;
-                const u64 key = ((u64)o[e] << 32) | (uint32_t)~(uint32_t)(j - lead);
-                uint32_t todo = __ballot_sync(0xffffffffu, o[e] != 0u && o[e] >= coarse && key > least);
-                while (todo) {
-                    const u64 next = __shfl_sync(0xffffffffu, key, __ffs(todo) - 1);
-                    todo &= todo - 1;
-                    if (next <= least) continue;            // (the list has grown since the ballot)
-                    const int at = __popc(__ballot_sync(0xffffffffu, list > next));
-                    const u64 up = __shfl_up_sync(0xffffffffu, list, 1);
-                    list = lane < at ? list : lane == at ? next : up;
-                    least = __shfl_sync(0xffffffffu, list, beams - 1);
-                }
-            }
-        }
-    }
-    // the lanes' sums, then the warps' lists and sums
-    const float warp_top = warp_max(top);
-    sum = warp_sum(warp_top == -INFINITY ? 0.f : sum * exp2f((top - warp_top) * log2e));
+// The 32 largest keys of the CTA's warps, sorted downwards over the lanes of warp 0, from lists that are so in every warp.
+__device__ __forceinline__ u64 merge_warps(u64 list, u64 (&meet)[ROW_WARPS][32], int warp, int lane) {
     meet[warp][lane] = list;
-    if (lane == 0) { meet_max[warp] = warp_top; meet_sum[warp] = sum; }
 #pragma unroll
     for (int half = ROW_WARPS / 2; half > 0; half >>= 1) {
         __syncthreads();
@@ -154,10 +85,122 @@ beam_rows_kernel(const float* __restrict__ logits, const int* __restrict__ ended
             meet[warp][lane] = list;
         }
     }
+    return list;
+}
+
+__global__ void __launch_bounds__(ROW_THREADS)
+beam_rows_kernel(const float* __restrict__ logits, const int* __restrict__ ended, u64* __restrict__ lists, float* __restrict__ sums,
+                 int vocab, int limit, int beams, int chunk) {
+    __shared__ u64 meet[ROW_WARPS][32], lanes_in_order[32];
+    __shared__ float meet_max[ROW_WARPS], meet_sum[ROW_WARPS];
+    const int row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_wait();
+    pdl_trigger();
+    if (ended != nullptr && ended[row] != 0) return;       // its one candidate is itself
+    const float* const base = logits + (size_t)row * vocab;
+    // ids are counted from the 16-byte boundary at or in front of the row's first logit
+    const int lead = (int)(((uintptr_t)base >> 2) & 3);
+    const int begin = (blockIdx.x * ROW_WARPS + warp) * chunk, end = min(limit + lead, begin + chunk);
+    const float log2e = 1.4426950408889634f;
+    // One pass for the sums and every lane's largest logit (16 a batch and lane, four neighbours at a time; what is not there, or
+    // no number, is minus infinity).
+    auto quad = [&](int at, float (&x)[4]) {
+        if (at >= lead && at + 4 <= end) {
+            const float4 v = *reinterpret_cast<const float4*>(base + (at - lead));
+            x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = (at + i >= lead && at + i < end) ? base[at + i - lead] : -INFINITY;
+        }
+    };
+    float top = -INFINITY, sum = 0.f, next_x[4][4];
+    int top_batch = begin;
+    if (begin < end)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) quad(begin + q * 128 + lane * 4, next_x[q]);
+    for (int b0 = begin; b0 < end; b0 += BATCH) {
+        float x[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = fmaxf(next_x[e >> 2][e & 3], -INFINITY);
+        if (b0 + BATCH < end)                               // on its way while these are looked at
+#pragma unroll
+            for (int q = 0; q < 4; ++q) quad(b0 + BATCH + q * 128 + lane * 4, next_x[q]);
+        float high = x[0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) high = fmaxf(high, x[e]);
+        if (high > top) {                                   // the sum is relative to the largest so far
+            sum *= exp2f((top - high) * log2e);
+            top = high;
+            top_batch = b0;
+        }
+        const float shift = top == -INFINITY ? 0.f : top * log2e;
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 16; ++e) part[e & 3] += exp2_approx(fmaf(x[e], log2e, -shift));
+        sum += (part[0] + part[1]) + (part[2] + part[3]);
+    }
+    const float warp_top = warp_max(top);
+    sum = warp_sum(warp_top == -INFINITY ? 0.f : sum * exp2f((top - warp_top) * log2e));
+    if (lane == 0) { meet_max[warp] = warp_top; meet_sum[warp] = sum; }
+    // The key of the lane's largest logit: the first of its batch that is as large.
+    u64 key = 0;
+#pragma unroll
+    for (int q = 3; q >= 0; --q) {
+        float x[4];
+        const int at = top_batch + q * 128 + lane * 4;
+        quad(at, x);
+#pragma unroll
+        for (int i = 3; i >= 0; --i)
+            if (at + i >= lead && at + i < end && fmaxf(x[i], -INFINITY) == top) key = key_of(top, at + i - lead);
+    }
+    // The CTA's 256 lanes have `beams` logits not below the beams-th largest of those: what is as good lies in the lanes of the
+    // first `beams` of them (all keys differ), whose logits are looked at once more, a lane's by a warp.
+    const u64 best_lane = merge_warps(sort_lanes(key, lane), meet, warp, lane);
+    if (warp == 0) lanes_in_order[lane] = best_lane;
+    __syncthreads();
+    const u64 bound = lanes_in_order[beams - 1];
+    u64 list = 0, least = 0;                                // lane i: the warp's i-th best; its beams-th best
+    for (int k = warp; k < beams; k += ROW_WARPS) {
+        const u64 owner = lanes_in_order[k];
+        if (owner == 0) break;
+        const int cta = blockIdx.x * ROW_WARPS * chunk, at = (int)~(uint32_t)owner + lead - cta;      // where the lane's best lies
+        const int first = cta + at / chunk * chunk, column = first + at % chunk % 128 / 4 * 4, last = min(limit + lead, first + chunk);
+        for (int q = lane; q < chunk / 128 + lane; q += 32) {      // (whole warps)
+            const int j = column + q * 128;
+            float x[4];
+            const bool there = q < chunk / 128;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = -INFINITY;
+            if (there && j >= lead && j + 4 <= last) {
+                const float4 v = *reinterpret_cast<const float4*>(base + (j - lead));
+                x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+            } else if (there) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (j + i >= lead && j + i < last) x[i] = base[j + i - lead];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const u64 mine = there && j + i >= lead && j + i < last ? key_of(fmaxf(x[i], -INFINITY), j + i - lead) : 0;
+                uint32_t todo = __ballot_sync(0xffffffffu, mine != 0 && mine >= bound && mine > least);
+                while (todo) {
+                    const u64 next = __shfl_sync(0xffffffffu, mine, __ffs(todo) - 1);
+                    todo &= todo - 1;
+                    if (next <= least) continue;            // (the list has grown since the ballot)
+                    const int place = __popc(__ballot_sync(0xffffffffu, list > next));
+                    const u64 up = __shfl_up_sync(0xffffffffu, list, 1);
+                    list = lane < place ? list : lane == place ? next : up;
+                    least = __shfl_sync(0xffffffffu, list, beams - 1);
+                }
+            }
+        }
+    }
+    __syncthreads();                                        // (the lanes' lists have been read)
+    list = merge_warps(list, meet, warp, lane);
     if (warp == 0) {
         const size_t at = (size_t)row * gridDim.x + blockIdx.x;
         if (lane < beams) lists[at * beams + lane] = list;
-        float m = lane < ROW_WARPS ? meet_max[lane] : -INFINITY;
+        const float m = lane < ROW_WARPS ? meet_max[lane] : -INFINITY;
         const float all = warp_max(m);
         const float s = warp_sum(lane < ROW_WARPS && all != -INFINITY ? meet_sum[lane] * exp2f((m - all) * log2e) : 0.f);
         if (lane == 0) *reinterpret_cast<float2*>(sums + at * 2) = make_float2(all, s);
@@ -182,78 +225,88 @@ struct ChoiceArgs {
 
 __global__ void __launch_bounds__(1024) beam_choice_kernel(const __grid_constant__ ChoiceArgs a) {
     __shared__ u64 meet[32][32];                         // lists of the warps, then the candidates' ranks [row][order]
-    __shared__ double value[32][32];
-    __shared__ int token[32][32], row_length[32], row_over[32];
+    __shared__ double value[32][32], row_total[32], row_weight[32];
+    __shared__ int token[32][32], row_length[32], row_over[32], choice[32];
     const int group = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-    const int per_row = warps / a.in_beams;               // warps that share a row's lists
+    const int per_row = warps / a.in_beams;               // warps that share a row's lists, a power of two
     const int b = warp / per_row, share = warp - b * per_row;
-    pdl_trigger();
+    const int row = group * a.in_beams + b;
+    // (the row's first warp ends up with its list; the last one works out what the logits are measured against meanwhile)
+    const bool leads = share == 0, sums_up = share == per_row - 1;
     pdl_wait();
-    const bool works = b < a.in_beams;
-    const int row = group * a.in_beams + (works ? b : 0);
+    pdl_trigger();
     const bool over = a.ended != nullptr && a.ended[row] != 0;
+    const double before = (double)a.scores[row];
+    const int length = (a.lengths != nullptr ? max(0, a.lengths[row]) : 0) + (over ? 0 : 1);
     u64 list = 0;
-    if (works && !over)
+    if (!over)
         for (int i = share; i < a.parts; i += per_row)
             list = merge_lists(list, lane < a.beams ? a.lists[((size_t)row * a.parts + i) * a.beams + lane] : 0, lane);
-    meet[warp][lane] = list;
-    __syncthreads();
-    if (works && share == 0) {
-        for (int i = 1; i < per_row; ++i) list = merge_lists(list, meet[warp + i][lane], lane);
-        const double before = (double)a.scores[row];
-        int length = a.lengths != nullptr ? max(0, a.lengths[row]) : 0;
-        double v = -INFINITY;
-        int t = a.end_token;
-        if (over) {
-            if (lane == 0) v = before;
-        } else {
-            ++length;
-            float m = -INFINITY;
-            for (int i = lane; i < a.parts; i += 32) m = fmaxf(m, a.sums[((size_t)row * a.parts + i) * 2]);
-            m = warp_max(m);
-            double s = 0.0;
-            for (int i = lane; i < a.parts; i += 32) {
-                const float2 ms = *reinterpret_cast<const float2*>(a.sums + ((size_t)row * a.parts + i) * 2);
-                if (ms.x != -INFINITY) s += (double)ms.y * (double)exp2f((ms.x - m) * 1.4426950408889634f);
+    if (sums_up) {
+        double total = 0.0;
+        if (!over) {
+            // the sums, relative to the largest maximum
+            float2 ms = lane < a.parts ? *reinterpret_cast<const float2*>(a.sums + ((size_t)row * a.parts + lane) * 2) : make_float2(-INFINITY, 0.f);
+            for (int i = lane + 32; i < a.parts; i += 32) {
+                const float2 more = *reinterpret_cast<const float2*>(a.sums + ((size_t)row * a.parts + i) * 2);
+                const float high = fmaxf(ms.x, more.x);
+                if (high != -INFINITY)
+                    ms.y = ms.y * exp2f((ms.x - high) * 1.4426950408889634f) + more.y * exp2f((more.x - high) * 1.4426950408889634f);
+                ms.x = high;
             }
+            const float m = warp_max(ms.x);
+            double s = ms.x != -INFINITY ? (double)ms.y * (double)exp2f((ms.x - m) * 1.4426950408889634f) : 0.0;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            v = before + ((double)number_of((uint32_t)(list >> 32)) - ((double)m + log(s)));
-            t = (int)~(uint32_t)list;
-        }
-        if (!(v == v)) v = -INFINITY;
-        const double weighed = a.penalty == 0.0 ? v : v / pow((double)max(1, length), a.penalty);
-        if (lane < a.beams) {
-            value[b][lane] = v;
-            token[b][lane] = t;
+            total = (double)m + log(s);
         }
         if (lane == 0) {
+            row_total[b] = total;
+            row_weight[b] = a.penalty == 0.0 ? 1.0 : a.penalty == 1.0 ? (double)max(1, length) : pow((double)max(1, length), a.penalty);
             row_length[b] = length;
             row_over[b] = over;
         }
-        list = lane < a.beams ? order_of(weighed == weighed ? weighed : -INFINITY) : 0;
     }
-    __syncthreads();                                      // the lists are read: their place is free
-    if (works && share == 0) meet[b][lane] = list;
+    for (int half = per_row >> 1; half > 0; half >>= 1) {
+        if (share >= half && share < 2 * half) meet[warp][lane] = list;
+        __syncthreads();
+        if (share < half) list = merge_lists(list, meet[warp + half][lane], lane);
+        __syncthreads();
+    }
+    if (per_row == 1) __syncwarp();
+    if (leads && lane < a.beams) {
+        double v = over ? (lane == 0 ? before : -INFINITY) : before + ((double)number_of((uint32_t)(list >> 32)) - row_total[b]);
+        if (!(v == v)) v = -INFINITY;
+        double weighed = v / row_weight[b];
+        if (!(weighed == weighed)) weighed = -INFINITY;
+        value[b][lane] = v;
+        token[b][lane] = over ? a.end_token : (int)~(uint32_t)list;
+        meet[b][lane] = order_of(weighed);
+    }
+    __syncthreads();
+    // A thread a candidate: its rank is its place in its own row and, in each other row, the number of candidates in front of it
+    // (equal ones of a lower row are), by bisection.
+    for (int c = threadIdx.x; c < a.in_beams * a.beams; c += blockDim.x) {
+        const int r = c / a.beams, order = c - r * a.beams;
+        const u64 mine = meet[r][order];
+        int rank = order;
+        for (int other = 0; other < a.in_beams; ++other) {
+            if (other == r) continue;
+            int lo = 0, hi = a.beams;                     // candidates of `other` that come first: [0, lo)
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                const u64 theirs = meet[other][mid];
+                if (theirs > mine || (theirs == mine && other < r)) lo = mid + 1; else hi = mid;
+            }
+            rank += lo;
+        }
+        if (rank < a.beams) choice[rank] = r * 32 + order;
+    }
     __syncthreads();
     if (warp != 0) return;
-    // lane b holds row b's first candidate that is not chosen yet; lane r remembers the r-th choice
-    int cursor = 0, from = 0, order = 0;
-    u64 head = lane < a.in_beams ? meet[lane][0] : 0;
-    for (int r = 0; r < a.beams; ++r) {
-        const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(head >> 32));
-        const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(head >> 32) == hi ? (uint32_t)head : 0u);
-        const u64 best = ((u64)hi << 32) | lo;
-        const int winner = __ffs(__ballot_sync(0xffffffffu, head == best)) - 1;
-        const int at = __shfl_sync(0xffffffffu, cursor, winner);
-        if (lane == r) { from = winner; order = at; }
-        if (lane == winner) {
-            ++cursor;
-            head = cursor < a.beams ? meet[lane][cursor] : 0;
-        }
-    }
     // rows: the best continuation of a beam takes its row, the others the rows that are left, in order
     const bool chosen = lane < a.beams;
+    const int from = chosen ? choice[lane] >> 5 : 0, order = chosen ? choice[lane] & 31 : 0;
     const uint32_t same = __match_any_sync(0xffffffffu, chosen ? from : 32 + lane);
     const bool stays = chosen && (same & ((1u << lane) - 1u)) == 0u;
     const uint32_t taken = __reduce_or_sync(0xffffffffu, stays ? 1u << from : 0u);
@@ -313,7 +366,18 @@ struct ReorderArgs {
 
 template <typename V>
 __device__ __forceinline__ void move_run(char* to, const char* of, long long bytes, long long at, long long step) {
-    for (long long i = at * sizeof(V); i < bytes; i += step * sizeof(V)) *reinterpret_cast<V*>(to + i) = *reinterpret_cast<const V*>(of + i);
+    // several pieces on their way before the first is stored
+    constexpr int U = sizeof(V) == 16 ? 4 : 8;
+    const long long n = bytes / (long long)sizeof(V);
+    for (long long i = at; i < n; i += U * step) {
+        V v[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k)
+            if (i + k * step < n) v[k] = reinterpret_cast<const V*>(of)[i + k * step];
+#pragma unroll
+        for (int k = 0; k < U; ++k)
+            if (i + k * step < n) reinterpret_cast<V*>(to)[i + k * step] = v[k];
+    }
 }
 
 __device__ __forceinline__ void move_bytes(char* to, const char* of, long long bytes, int unit, long long at, long long step) {
@@ -325,17 +389,17 @@ __device__ __forceinline__ void move_bytes(char* to, const char* of, long long b
 }
 
 // CTA (piece, row, tensor): rows whose parent is another row take over what is the parent's.
-__global__ void __launch_bounds__(256) beam_reorder_kernel(const __grid_constant__ ReorderArgs a) {
+__global__ void __launch_bounds__(256, 4) beam_reorder_kernel(const __grid_constant__ ReorderArgs a) {
     pdl_trigger();
     pdl_wait();
     const int row = blockIdx.y;
-    const int parent = a.parents[row];
+    const int parent = a.parents[row], which = blockIdx.z;
     if (parent == row || parent < 0 || parent >= a.rows) return;
-    if (a.parents[parent] != parent) return;              // (the parent takes over another row itself: see above)
-    const int which = blockIdx.z;
+    const int grand = a.parents[parent], length = which < a.n_paged ? a.lengths[parent] : 0;
+    if (grand != parent) return;                          // (the parent takes over another row itself: see above)
     if (which < a.n_paged) {
         const Paged& p = a.paged[which];
-        const int length = a.lengths[parent], full = length / p.page_tokens, used = length - full * p.page_tokens;
+        const int full = length / p.page_tokens, used = length - full * p.page_tokens;
         int* const mine = p.table + (size_t)row * p.width;
         const int* const theirs = p.table + (size_t)parent * p.width;
         if (length <= 0) return;
@@ -395,9 +459,19 @@ MG_API int mg_beam_select(const float* logits, const float* scores, const int* e
     MG_CHECK_LAUNCH("beam_select");
     const ChoiceArgs a = {lists, sums, scores, ended, lengths, tokens, parents, scores_out, ranks, ended_out, lengths_out,
                           in_beams, beams, parts, end_token, penalty};
-    int per_row = 32 / in_beams;
-    if (per_row > parts) per_row = parts;
-    e = mg_launch(beam_choice_kernel, dim3(groups), dim3(32 * per_row * in_beams), 0, s, true, a);
+    int per_row = 1;
+    while (2 * per_row * in_beams <= 32 && per_row < parts) per_row *= 2;
+    // (it may start while the kernel in front of it, this operator's own, still runs)
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(groups);
+    cfg.blockDim = dim3(32 * per_row * in_beams);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, beam_choice_kernel, a);
     if (e != cudaSuccess) return mg_set_error(MG_ERR_CUDA, "beam_select (choice): %s", cudaGetErrorString(e));
     MG_CHECK_LAUNCH("beam_select (choice)");
     return MG_OK;
@@ -407,11 +481,11 @@ MG_API int mg_beam_select(const float* logits, const float* scores, const int* e
 // part-filled page (into the row's own page of that column), and the state slot's contents.  parents, lengths, slots: [rows]
 // ints on the device (lengths: tokens in the cache; slots may be null without states).  A parent has to be its own parent, as
 // mg_beam_select leaves them: rows with another parent are left alone, as are rows whose parent is out of range or whose page
-// is missing.  sizes: per paged group (layers, pages, kv heads, page tokens, bytes of a key, bytes of a value, table width);
-// v null: values live in the keys.  state_bytes, state_slots: per state tensor.
-MG_API int mg_beam_reorder(const int* parents, const int* lengths, const int* slots, int rows, int n_paged, void* const* tables,
-                           void* const* k, void* const* v, const int* sizes, int n_states, void* const* states,
-                           const long long* state_bytes, const int* state_slots, void* stream) {
+// is missing.
+// paged: per group ten numbers (addresses of table, keys and values, layers, pages, kv heads, page tokens, bytes of a key, bytes
+// of a value, table width); values 0: they live in the keys.  states: per tensor three (address, bytes of a slot, slots).
+MG_API int mg_beam_reorder(const int* parents, const int* lengths, const int* slots, int rows, int n_paged, int n_states,
+                           const long long* paged, const long long* states, void* stream) {
     if (rows == 0 || n_paged + n_states == 0) return MG_OK;
     MG_REQUIRE(rows > 0 && rows <= 65535 && n_paged >= 0 && n_paged <= MAX_PAGED && n_states >= 0 && n_states <= MAX_STATES,
                "beam_reorder: at most 65535 rows, %d groups of pages and %d states", MAX_PAGED, MAX_STATES);
@@ -420,21 +494,23 @@ MG_API int mg_beam_reorder(const int* parents, const int* lengths, const int* sl
     a.parents = parents; a.lengths = lengths; a.slots = slots; a.rows = rows; a.n_paged = n_paged; a.n_states = n_states;
     long long largest = 1;
     for (int g = 0; g < n_paged; ++g) {
-        const int* z = sizes + 7 * g;
-        MG_REQUIRE(z[0] > 0 && z[1] > 0 && z[2] > 0 && z[3] > 0 && z[4] > 0 && z[5] > 0 && z[6] > 0, "beam_reorder: bad page sizes");
+        const long long* z = paged + 10 * g;
+        for (int i = 3; i < 10; ++i) MG_REQUIRE(z[i] > 0 && z[i] < (1ll << 31), "beam_reorder: bad page sizes");
         Paged& p = a.paged[g];
-        p.table = (int*)tables[g]; p.k = (char*)k[g]; p.v = (char*)v[g];
-        p.layers = z[0]; p.num_pages = z[1]; p.n_kv_head = z[2]; p.page_tokens = z[3]; p.k_token = z[4]; p.v_token = z[5]; p.width = z[6];
-        p.k_layer = (long long)z[1] * z[2] * z[3] * z[4];
-        p.v_layer = (long long)z[1] * z[2] * z[3] * z[5];
+        p.table = (int*)z[0]; p.k = (char*)z[1]; p.v = (char*)z[2];
+        p.layers = (int)z[3]; p.num_pages = (int)z[4]; p.n_kv_head = (int)z[5]; p.page_tokens = (int)z[6];
+        p.k_token = (int)z[7]; p.v_token = (int)z[8]; p.width = (int)z[9];
+        p.k_layer = z[4] * z[5] * z[6] * z[7];
+        p.v_layer = z[4] * z[5] * z[6] * z[8];
         p.unit = unit_of((uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)p.k_token | (uintptr_t)p.v_token);
-        const long long bytes = (long long)z[0] * z[2] * z[3] * (z[4] + (p.v ? z[5] : 0));
+        const long long bytes = z[3] * z[5] * z[6] * (z[7] + (p.v ? z[8] : 0));
         if (bytes > largest) largest = bytes;
     }
     for (int i = 0; i < n_states; ++i) {
-        MG_REQUIRE(state_bytes[i] > 0 && state_slots[i] > 0, "beam_reorder: bad state sizes");
-        a.state[i] = {(char*)states[i], state_bytes[i], unit_of((uintptr_t)states[i] | (uintptr_t)state_bytes[i]), state_slots[i]};
-        if (state_bytes[i] > largest) largest = state_bytes[i];
+        const long long* z = states + 3 * i;
+        MG_REQUIRE(z[1] > 0 && z[2] > 0 && z[2] < (1ll << 31), "beam_reorder: bad state sizes");
+        a.state[i] = {(char*)z[0], z[1], unit_of((uintptr_t)z[0] | (uintptr_t)z[1]), (int)z[2]};
+        if (z[1] > largest) largest = z[1];
     }
     long long pieces = (largest + 32767) / 32768;
     if (pieces > 64) pieces = 64;

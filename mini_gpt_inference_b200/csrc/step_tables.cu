@@ -106,12 +106,12 @@ __global__ void __launch_bounds__(THREADS) step_tables_kernel(const __grid_const
 
 }  // namespace
 
-// rows (or null), before, fresh: [n_requests] ints on the device; per group g of n_groups (at most 8): pools[g]
-// [pool_rows, widths[g]] pages (below zero: none), tables[g] [n_requests, widths[g]], slots[g] [n_tokens].  Token rows behind
-// the last request's are padding: position and slots -1, request 0.  A request number of new tokens below zero counts as none.
+// rows (or null), before, fresh: [n_requests] ints on the device.  groups: per group of n_groups (at most 8) five numbers: the
+// addresses of its pages [pool_rows, width] (below zero: none), of the block tables [n_requests, width] and of the cache rows
+// [n_tokens] to be written, width, and tokens of a page.  Token rows behind the last request's are padding: position and cache
+// row -1, request 0.  A number of new tokens below zero counts as none.
 MG_API int mg_step_tables(const int* rows, const int* before, const int* fresh, int* token_request, int* positions, int* q_start,
-                          int n_requests, int n_tokens, int pool_rows, int n_groups, const void* const* pools, void* const* tables,
-                          void* const* slots, const int* widths, const int* page_tokens, void* stream) {
+                          int n_requests, int n_tokens, int pool_rows, int n_groups, const long long* groups, void* stream) {
     if (n_requests == 0 && n_tokens == 0) return MG_OK;
     MG_REQUIRE(n_requests > 0 && n_tokens >= 0 && pool_rows > 0 && n_groups >= 0, "step_tables: bad sizes");
     MG_REQUIRE(n_requests <= MAX_REQUESTS && n_groups <= MAX_GROUPS, "step_tables: at most %d requests and %d groups", MAX_REQUESTS, MAX_GROUPS);
@@ -119,8 +119,9 @@ MG_API int mg_step_tables(const int* rows, const int* before, const int* fresh, 
     a.rows = rows; a.before = before; a.fresh = fresh; a.token_request = token_request; a.positions = positions; a.q_start = q_start;
     a.n_requests = n_requests; a.n_tokens = n_tokens; a.pool_rows = pool_rows; a.n_groups = n_groups;
     for (int g = 0; g < n_groups; ++g) {
-        MG_REQUIRE(widths[g] > 0 && page_tokens[g] > 0, "step_tables: bad page sizes");
-        a.group[g] = {(const int*)pools[g], (int*)tables[g], (int*)slots[g], widths[g], page_tokens[g]};
+        const long long* z = groups + 5 * g;
+        MG_REQUIRE(z[3] > 0 && z[3] < (1ll << 31) && z[4] > 0 && z[4] < (1ll << 31), "step_tables: bad page sizes");
+        a.group[g] = {(const int*)z[0], (int*)z[1], (int*)z[2], (int)z[3], (int)z[4]};
     }
     int ctas = ceil_div(n_tokens, THREADS) > n_requests ? ceil_div(n_tokens, THREADS) : n_requests;
     if (ctas > 296) ctas = 296;

@@ -110,8 +110,8 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _pointers(tensors):
-    return (ctypes.c_void_p * len(tensors))(*(_ptr(t) for t in tensors))
+def _numbers(values):
+    return (ctypes.c_longlong * len(values))(*values)
 
 
 class CudaOps:
@@ -1906,32 +1906,30 @@ class CudaOps:
             raise KernelLibraryError("beam_reorder: one block table, keys and values per group of pages")
         if block_tables and self._want(lengths, torch.int32, "lengths", 1).numel() != rows:
             raise KernelLibraryError("beam_reorder: one length per row")
-        sizes = []
+        paged = []
         for table, k, v in zip(block_tables, k_pages, v_pages):
             if self._want(table, torch.int32, "block_table", 2).shape[0] != rows:
                 raise KernelLibraryError("beam_reorder: one row of the block table per row")
-            self._want(k, None, "k_pages")
-            if k.dim() not in (4, 5) or (v is not None and (self._want(v, k.dtype, "v_pages").shape[:-1] != k.shape[:-1])):
+            shape = self._want(k, None, "k_pages").shape
+            if len(shape) not in (4, 5) or (v is not None and self._want(v, k.dtype, "v_pages").shape[:-1] != shape[:-1]):
                 raise KernelLibraryError("beam_reorder: keys and values of shapes that do not fit")
-            layers, (pages, heads, page_tokens, size) = (k.shape[0] if k.dim() == 5 else 1), k.shape[-4:]
-            if v is not None and v.data_ptr() == k.data_ptr():
-                v = None
-            size *= k.element_size()
-            sizes += [layers, pages, heads, page_tokens, size, v.shape[-1] * v.element_size() if v is not None else size, table.shape[1]]
+            layers, (pages, heads, page_tokens, size), each = (shape[0] if len(shape) == 5 else 1), shape[-4:], k.element_size()
+            at_k, at_v, v_size = k.data_ptr(), 0 if v is None else v.data_ptr(), size if v is None else v.shape[-1]
+            paged += (table.data_ptr(), at_k, 0 if at_v == at_k else at_v, layers, pages, heads, page_tokens, size * each, v_size * each,
+                      table.shape[1])
         if states and (slots is None or self._want(slots, torch.int32, "slots", 1).numel() != rows):
             raise KernelLibraryError("beam_reorder: one state slot per row")
+        kept = []
         for state in states:
             if self._want(state, None, "state").dim() < 1 or state.shape[0] == 0:
                 raise KernelLibraryError("beam_reorder: a state without slots")
-        states = [s for s in states if s.numel()]
-        if rows == 0 or not (sizes or states):
+            if state.numel():
+                kept += (state.data_ptr(), state.numel() // state.shape[0] * state.element_size(), state.shape[0])
+        if rows == 0 or not (paged or kept):
             return
         self._run(self.lib.mg_beam_reorder(
-            _ptr(parents), _ptr(lengths), _ptr(slots), rows, len(block_tables), _pointers(block_tables), _pointers(k_pages),
-            _pointers([None if v is not None and v.data_ptr() == k.data_ptr() else v for k, v in zip(k_pages, v_pages)]),
-            (ctypes.c_int * len(sizes))(*sizes), len(states), _pointers(states),
-            (ctypes.c_longlong * len(states))(*(s.numel() // s.shape[0] * s.element_size() for s in states)),
-            (ctypes.c_int * len(states))(*(s.shape[0] for s in states)), self._stream()), "beam_reorder")
+            _ptr(parents), _ptr(lengths), _ptr(slots), rows, len(paged) // 10, len(kept) // 3, _numbers(paged), _numbers(kept),
+            self._stream()), "beam_reorder")
 
     def step_tables(self, pages, page_tokens, ctx_before, q_len, num_tokens, rows=None):
         """A step's integers from the lengths of its requests, on the device: request ``r`` has ``ctx_before[r]`` tokens in
@@ -1957,15 +1955,16 @@ class CudaOps:
             raise KernelLibraryError("step_tables: fewer rows of pages than requests")
         if R == 0:
             raise KernelLibraryError("step_tables: no requests")
-        per_token = torch.empty((2 + groups, n), dtype=torch.int32, device=self.device).unbind(0)
-        tables = [torch.empty((R, width), dtype=torch.int32, device=self.device) for width in widths]
-        out = StepTables(per_token[0], per_token[1], torch.empty((R,), dtype=torch.int32, device=self.device), tables,
-                         list(per_token[2:]))
-        ints = ctypes.c_int * groups
+        parts = [n] * (2 + groups) + [R] + [R * width for width in widths]
+        parts = torch.empty((sum(parts),), dtype=torch.int32, device=self.device).split(parts)
+        out = StepTables(parts[0], parts[1], parts[2 + groups], [t.view(R, width) for t, width in zip(parts[3 + groups:], widths)],
+                         list(parts[2: 2 + groups]))
+        numbers = []
+        for pool, table, slots, width, size in zip(pages, out.block_tables, out.slot_mapping, widths, page_tokens):
+            numbers += (pool.data_ptr(), table.data_ptr(), slots.data_ptr(), width, int(size))
         self._run(self.lib.mg_step_tables(
             _ptr(rows), _ptr(ctx_before), _ptr(q_len), _ptr(out.token_request), _ptr(out.positions), _ptr(out.req_q_start), R, n,
-            pool_rows, groups, _pointers(pages), _pointers(tables), _pointers(out.slot_mapping), ints(*widths),
-            ints(*(int(p) for p in page_tokens)), self._stream()), "step_tables")
+            pool_rows, groups, _numbers(numbers), self._stream()), "step_tables")
         return out
 
 
