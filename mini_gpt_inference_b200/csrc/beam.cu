@@ -12,8 +12,8 @@
 //                  from above: all keys differ, so ties need no care.  Lists are sorted over a warp's lanes and joined by
 //                  bitonic merges.  (Every warp keeping the B best of its piece as it reads: 768 instructions for 512 logits
 //                  of 50,257 and B = 16, and bound by them: 85 us for 64 x 16 rows.)
-//   choice kernel  one CTA a group: the rows' lists and sums joined, values in 64 bits, and a thread a candidate that counts
-//                  those in front of it.
+//   choice kernel  one CTA a group: the rows' lists and sums joined, values in 64 bits, and the candidates in front of each
+//                  counted.
 //
 // A beam that goes on stays in its row: its best continuation takes the row, its others take, in order of rank, the rows
 // whose beams do not go on.  So only those rows' caches change hands, a row that is read is never written (reorder needs
@@ -226,7 +226,7 @@ struct ChoiceArgs {
 __global__ void __launch_bounds__(1024) beam_choice_kernel(const __grid_constant__ ChoiceArgs a) {
     __shared__ u64 meet[32][32];                         // lists of the warps, then the candidates' ranks [row][order]
     __shared__ double value[32][32], row_total[32], row_weight[32];
-    __shared__ int token[32][32], row_length[32], row_over[32], choice[32];
+    __shared__ int token[32][32], rank[32][32], row_length[32], row_over[32], choice[32];
     const int group = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const int per_row = warps / a.in_beams;               // warps that share a row's lists, a power of two
     const int b = warp / per_row, share = warp - b * per_row;
@@ -282,26 +282,25 @@ __global__ void __launch_bounds__(1024) beam_choice_kernel(const __grid_constant
         value[b][lane] = v;
         token[b][lane] = over ? a.end_token : (int)~(uint32_t)list;
         meet[b][lane] = order_of(weighed);
+        rank[b][lane] = lane;
     }
     __syncthreads();
-    // A thread a candidate: its rank is its place in its own row and, in each other row, the number of candidates in front of it
-    // (equal ones of a lower row are), by bisection.
-    for (int c = threadIdx.x; c < a.in_beams * a.beams; c += blockDim.x) {
-        const int r = c / a.beams, order = c - r * a.beams;
+    // A candidate's rank is its place in its own row and, in each other row, the number of candidates in front of it (equal ones of
+    // a lower row are), by bisection: a thread a candidate and other row.
+    const int candidates = a.in_beams * a.beams;
+    for (int x = threadIdx.x; x < candidates * a.in_beams; x += blockDim.x) {
+        const int other = x / candidates, c = x - other * candidates, r = c / a.beams, order = c - r * a.beams;
         const u64 mine = meet[r][order];
-        int rank = order;
-        for (int other = 0; other < a.in_beams; ++other) {
-            if (other == r) continue;
-            int lo = 0, hi = a.beams;                     // candidates of `other` that come first: [0, lo)
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                const u64 theirs = meet[other][mid];
-                if (theirs > mine || (theirs == mine && other < r)) lo = mid + 1; else hi = mid;
-            }
-            rank += lo;
+        int lo = 0, hi = other == r ? 0 : a.beams;        // candidates of `other` that come first: [0, lo)
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            const u64 theirs = meet[other][mid];
+            if (theirs > mine || (theirs == mine && other < r)) lo = mid + 1; else hi = mid;
         }
-        if (rank < a.beams) choice[rank] = r * 32 + order;
+        if (lo > 0) atomicAdd(&rank[r][order], lo);
     }
+    __syncthreads();
+    if (leads && lane < a.beams && rank[b][lane] < a.beams) choice[rank[b][lane]] = b * 32 + lane;
     __syncthreads();
     if (warp != 0) return;
     // rows: the best continuation of a beam takes its row, the others the rows that are left, in order
