@@ -37,10 +37,12 @@ struct SharedArgs {
     float* part_out;                   // [row][head][slot][D]
     float* part_ml;                    // [row][head][slot][2]
     int* behind;                       // [row]: keys that its shared ranges hold (the ranges' kernel tells the joining one)
+    int element;                       // bytes of a number of `out`
     int n_groups, n, n_head, n_kv_head, D, page_tokens, max_pages, num_pages, n_requests;
     int row_tiles;                     // CTAs that share the (row, head) pairs of a group
     int shared_slots, own_slots;       // ranges of the shared keys, and of a row's own
     int shared_least;                  // keys of a range of shared keys, at least, and what they are a multiple of
+    int direct;                        // every row has one range alone: the results, not parts to be joined, are left
     int first_item;                    // item of the grid's first CTA: above 0 where another kernel takes the shared ranges
     float scale_log2e;
 };
@@ -110,7 +112,15 @@ __device__ __forceinline__ bool item_of(const SharedArgs& a, int item, Item& it)
         request = a.token_request[it.first_row];
         int behind = group_tokens(a, it.first_row);
         if (behind > p + 1) behind = 0;
-        if (it.slot == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.behind[it.first_row] = behind;
+        if (a.direct) {
+            if (p < 0) {                                  // padding of a fixed-size batch (else the joining kernel's work)
+                const int size = a.n_head / a.n_kv_head * a.D * a.element;
+                char* const out = (char*)a.out + ((size_t)it.first_row * a.n_kv_head + blockIdx.y) * size;
+                for (int i = threadIdx.x; i < size; i += blockDim.x) out[i] = 0;
+            }
+        } else if (it.slot == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
+            a.behind[it.first_row] = behind;
+        }
         const int step = range_keys(p + 1 - behind, a.own_slots, OWN_LEAST);
         it.key0 = behind + it.slot * step;
         it.key1 = min(p + 1, it.key0 + step);
@@ -138,79 +148,135 @@ __device__ __forceinline__ int pair_row(const SharedArgs& a, const Item& it, int
     return !it.shared || a.positions[row] + 1 >= it.shared_keys ? row : -1;
 }
 
-// ---- any head size, either type: 16 (row, head) pairs and 64 keys at a time, in 32-bit arithmetic ------------------------
-constexpr int SIMT_THREADS = 128, SIMT_QUERIES = 16;
+// What a range leaves of feature d of a (row, head): the unnormalised average, with the maximum and the sum, or, where a row has one
+// range alone, the result.
+template <typename T>
+__device__ __forceinline__ void leave(const SharedArgs& a, const Item& it, int row, int head, int d, float v, float top, float sum) {
+    const size_t pair = (size_t)row * a.n_head + head;
+    if (a.direct) {
+        ((T*)a.out)[pair * a.D + d] = from_float<T>(sum != 0.f ? v / sum : 0.f);      // (no key has a page: zeros)
+        return;
+    }
+    const size_t at = pair * (a.shared_slots + a.own_slots) + it.slot;
+    a.part_out[at * a.D + d] = v;
+    if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(top, sum);
+}
+
+// ---- any head size, either type: 8 or 16 (row, head) pairs and 64 keys at a time, in 32-bit arithmetic -------------------
+// The 32-bit mode's kernel, and that of bfloat16 heads whose size is no multiple of 8.  Keys and values of a block come to
+// shared memory together, several loads a thread on their way (read one by one where they are used: 27 us for 10 rows of
+// some 530 keys and 12 heads of 64, where this takes SIMT_US).  Scores: a thread a key and half of the pairs; average: a thread a
+// feature and all pairs.
+constexpr int SIMT_THREADS = 128;
 
 __host__ __device__ constexpr int simt_lanes(int d) { return d > 64 ? 128 : d > 32 ? 64 : 32; }     // threads across the features
 
-template <typename T>
+// Rows of a block into shared memory as 32-bit numbers; missing rows as zeros.  VEC: four features at a time.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_rows(const T* pages, const int* krow, float* to, int stride, int D) {
+    constexpr int W = VEC ? 4 : 1;
+    const int pieces = D / W, lanes = pieces > 16 ? 32 : pieces > 8 ? 16 : 8, at_once = SIMT_THREADS / lanes;
+    const int r0 = threadIdx.x / lanes, c0 = threadIdx.x % lanes;
+    for (int c = c0; c < pieces; c += lanes)
+#pragma unroll 4
+        for (int r = r0; r < BLOCK_KEYS; r += at_once) {
+            const int row = krow[r];
+            float v[W];
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[i] = 0.f;
+            if (row >= 0) {
+                const T* from = pages + (size_t)row * D + c * W;
+                if constexpr (VEC) {
+                    const float4 x = *reinterpret_cast<const float4*>(from);
+                    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+                } else {
+                    v[0] = to_float(*from);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < W; ++i) to[r * stride + c * W + i] = v[i];
+        }
+}
+
+template <typename T, int NQ, bool VEC>
 __global__ void __launch_bounds__(SIMT_THREADS) attention_shared_simt_kernel(SharedArgs a) {
-    extern __shared__ float smem[];
-    __shared__ int krow[BLOCK_KEYS], q_token[SIMT_QUERIES], q_head[SIMT_QUERIES];
-    __shared__ float q_max[SIMT_QUERIES], q_sum[SIMT_QUERIES], q_corr[SIMT_QUERIES];
+    extern __shared__ float4 smem4[];
+    __shared__ int krow[BLOCK_KEYS], q_token[NQ], q_head[NQ];
+    __shared__ float q_max[NQ], q_sum[NQ], q_corr[NQ];
+    constexpr int HALF = NQ / 2;
     const int tid = threadIdx.x, D = a.D, kv_head = blockIdx.y, share = a.n_head / a.n_kv_head;
-    float* q_s = smem;                                   // [D][16]
-    float* k_s = q_s + D * SIMT_QUERIES;                 // [64][D + 1]
-    float* p_s = k_s + BLOCK_KEYS * (D + 1);             // [64][16]
+    float* q_s = reinterpret_cast<float*>(smem4);        // [D][NQ]
+    float* p_s = q_s + D * NQ;                           // [64][NQ]
+    float* v_s = p_s + BLOCK_KEYS * NQ;                  // [64][D]
+    float* k_s = v_s + BLOCK_KEYS * D;                   // [64][D + 1]
     const int lanes = simt_lanes(D), dl = tid % lanes, ks = tid / lanes, key_parts = SIMT_THREADS / lanes;
 
     Item it;
     pdl_wait();
     pdl_trigger();
     if (!item_of(a, a.first_item + blockIdx.x, it)) return;
-    for (int q0 = it.tile * SIMT_QUERIES; q0 < it.rows * share; q0 += it.tiles * SIMT_QUERIES) {
+    for (int q0 = it.tile * NQ; q0 < it.rows * share; q0 += it.tiles * NQ) {
         __syncthreads();
-        if (tid < SIMT_QUERIES) {
+        if (tid < NQ) {
             q_token[tid] = pair_row(a, it, q0 + tid, share);
             q_head[tid] = kv_head * share + (q0 + tid) % share;
             q_max[tid] = -INFINITY;
             q_sum[tid] = 0.f;
         }
         __syncthreads();
-        for (int i = tid; i < SIMT_QUERIES * D; i += SIMT_THREADS) {
-            const int j = i / D, d = i - j * D;
-            q_s[d * SIMT_QUERIES + j] =
-                q_token[j] < 0 ? 0.f : to_float(((const T*)a.q)[q_token[j] * a.q_stride + (size_t)q_head[j] * D + d]) * a.scale_log2e;
-        }
-        float acc[2][SIMT_QUERIES];
+        for (int d = tid; d < D; d += SIMT_THREADS)
+#pragma unroll
+            for (int j = 0; j < NQ; ++j)
+                q_s[d * NQ + j] = q_token[j] < 0 ? 0.f : to_float(((const T*)a.q)[q_token[j] * a.q_stride + (size_t)q_head[j] * D + d]) * a.scale_log2e;
+        float acc[2][NQ];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int j = 0; j < SIMT_QUERIES; ++j) acc[i][j] = 0.f;
+            for (int j = 0; j < NQ; ++j) acc[i][j] = 0.f;
         for (int b0 = it.key0; b0 < it.key1; b0 += BLOCK_KEYS) {
             __syncthreads();
             if (tid < BLOCK_KEYS) krow[tid] = cache_row(a, it, b0 + tid, kv_head);
             __syncthreads();
-            for (int i = tid; i < BLOCK_KEYS * D; i += SIMT_THREADS) {
-                const int r = i / D, d = i - r * D;
-                k_s[r * (D + 1) + d] = krow[r] < 0 ? 0.f : to_float(((const T*)a.k_pages)[(size_t)krow[r] * D + d]);
-            }
+            load_rows<T, VEC>((const T*)a.k_pages, krow, k_s, D + 1, D);
+            load_rows<T, VEC>((const T*)a.v_pages, krow, v_s, D, D);
             __syncthreads();
             {
-                const int key = tid & (BLOCK_KEYS - 1), j0 = (tid / BLOCK_KEYS) * 8;
-                float s[8];
+                const int key = tid & (BLOCK_KEYS - 1), j0 = (tid / BLOCK_KEYS) * HALF;
+                float s[HALF];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) s[j] = 0.f;
+                for (int j = 0; j < HALF; ++j) s[j] = 0.f;
+#pragma unroll 4
                 for (int d = 0; d < D; ++d) {
                     const float k = k_s[key * (D + 1) + d];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) s[j] = fmaf(k, q_s[d * SIMT_QUERIES + j0 + j], s[j]);
+                    for (int j = 0; j < HALF; j += 4) {
+                        const float4 q = *reinterpret_cast<const float4*>(q_s + d * NQ + j0 + j);
+                        s[j] = fmaf(k, q.x, s[j]);
+                        s[j + 1] = fmaf(k, q.y, s[j + 1]);
+                        s[j + 2] = fmaf(k, q.z, s[j + 2]);
+                        s[j + 3] = fmaf(k, q.w, s[j + 3]);
+                    }
                 }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) p_s[key * SIMT_QUERIES + j0 + j] = krow[key] < 0 ? -INFINITY : s[j];
+                for (int j = 0; j < HALF; ++j) p_s[key * NQ + j0 + j] = krow[key] < 0 ? -INFINITY : s[j];
             }
             __syncthreads();
-            {
+            if (tid < NQ * 8) {
                 const int j = tid >> 3, part = tid & 7;              // eight neighbouring threads a query
-                float m = -INFINITY;
-                for (int k = part; k < BLOCK_KEYS; k += 8) m = fmaxf(m, p_s[k * SIMT_QUERIES + j]);
+                float x[BLOCK_KEYS / 8], m = -INFINITY;
+#pragma unroll
+                for (int k = 0; k < BLOCK_KEYS / 8; ++k) {
+                    x[k] = p_s[(k * 8 + part) * NQ + j];
+                    m = fmaxf(m, x[k]);
+                }
 #pragma unroll
                 for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
                 const float before = q_max[j], top = fmaxf(before, m);
                 float sum = 0.f;
-                for (int k = part; k < BLOCK_KEYS; k += 8) {
-                    const float e = top == -INFINITY ? 0.f : exp2f(p_s[k * SIMT_QUERIES + j] - top);
-                    p_s[k * SIMT_QUERIES + j] = e;
+#pragma unroll
+                for (int k = 0; k < BLOCK_KEYS / 8; ++k) {
+                    const float e = top == -INFINITY ? 0.f : exp2f(x[k] - top);
+                    p_s[(k * 8 + part) * NQ + j] = e;
                     sum += e;
                 }
 #pragma unroll
@@ -227,16 +293,22 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_shared_simt_kernel(Sha
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int j = 0; j < SIMT_QUERIES; ++j) acc[i][j] *= q_corr[j];
-            for (int k = ks; k < BLOCK_KEYS; k += key_parts) {
-                if (krow[k] < 0) continue;
+                for (int j = 0; j < NQ; ++j) acc[i][j] *= q_corr[j];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int d = dl + i * SIMT_THREADS;
-                    if (d >= D) break;
-                    const float v = to_float(((const T*)a.v_pages)[(size_t)krow[k] * D + d]);
+            for (int i = 0; i < 2; ++i) {
+                const int d = dl + i * SIMT_THREADS;
+                if (d >= D) break;
+#pragma unroll 4
+                for (int k = ks; k < BLOCK_KEYS; k += key_parts) {
+                    const float v = v_s[k * D + d];
 #pragma unroll
-                    for (int j = 0; j < SIMT_QUERIES; ++j) acc[i][j] = fmaf(p_s[k * SIMT_QUERIES + j], v, acc[i][j]);
+                    for (int j = 0; j < NQ; j += 4) {
+                        const float4 p = *reinterpret_cast<const float4*>(p_s + k * NQ + j);
+                        acc[i][j] = fmaf(p.x, v, acc[i][j]);
+                        acc[i][j + 1] = fmaf(p.y, v, acc[i][j + 1]);
+                        acc[i][j + 2] = fmaf(p.z, v, acc[i][j + 2]);
+                        acc[i][j + 3] = fmaf(p.w, v, acc[i][j + 3]);
+                    }
                 }
             }
         }
@@ -245,23 +317,20 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_shared_simt_kernel(Sha
             __syncthreads();
             if (ks > 0 && dl < D)
 #pragma unroll
-                for (int j = 0; j < SIMT_QUERIES; ++j) k_s[((ks - 1) * SIMT_QUERIES + j) * D + dl] = acc[0][j];
+                for (int j = 0; j < NQ; ++j) k_s[((ks - 1) * NQ + j) * D + dl] = acc[0][j];
             __syncthreads();
             if (ks == 0 && dl < D)
                 for (int other = 0; other < key_parts - 1; ++other)
 #pragma unroll
-                    for (int j = 0; j < SIMT_QUERIES; ++j) acc[0][j] += k_s[(other * SIMT_QUERIES + j) * D + dl];
+                    for (int j = 0; j < NQ; ++j) acc[0][j] += k_s[(other * NQ + j) * D + dl];
         }
-        const int slots = a.shared_slots + a.own_slots;
         if (ks == 0)
 #pragma unroll
-            for (int j = 0; j < SIMT_QUERIES; ++j) {
+            for (int j = 0; j < NQ; ++j) {
                 if (q_token[j] < 0) continue;
-                const size_t at = ((size_t)q_token[j] * a.n_head + q_head[j]) * slots + it.slot;
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    if (dl + i * SIMT_THREADS < D) a.part_out[at * D + dl + i * SIMT_THREADS] = acc[i][j];
-                if (dl == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(q_max[j], q_sum[j]);
+                    if (dl + i * SIMT_THREADS < D) leave<T>(a, it, q_token[j], q_head[j], dl + i * SIMT_THREADS, acc[i][j], q_max[j], q_sum[j]);
             }
     }
 }
@@ -500,7 +569,6 @@ __global__ void __launch_bounds__(MMA_THREADS) attention_shared_mma_kernel(Share
                 }
             }
         __syncthreads();
-        const int slots = a.shared_slots + a.own_slots;
         for (int e = tid; e < nts * 8 * DP; e += MMA_THREADS) {
             const int j = e / DP, d = e % DP, token = pair_row(a, it, q0 + j, share);
             if (token < 0 || d >= D) continue;
@@ -514,9 +582,7 @@ __global__ void __launch_bounds__(MMA_THREADS) attention_shared_mma_kernel(Share
                 v = fmaf(f, src[d], v);
                 l = fmaf(f, src[DP + 1], l);
             }
-            const size_t at = ((size_t)token * a.n_head + kv_head * share + (q0 + j) % share) * slots + it.slot;
-            a.part_out[at * D + d] = v;
-            if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(top, l);
+            leave<bf16>(a, it, token, kv_head * share + (q0 + j) % share, d, v, top, l);
         }
         __syncthreads();                                                // (the tiles are loaded again for the next pairs)
     }
@@ -975,6 +1041,8 @@ __global__ void __launch_bounds__(128) attention_shared_join_kernel(SharedArgs a
         if (lane + 32 * j < a.D) out[lane + 32 * j] = from_float<T>(acc[j] * inv);
 }
 
+int simt_pairs(int pairs) { return pairs <= 8 ? 8 : 16; }
+
 // A kernel that may start while the one in front of it, which is this operator's own, still runs.
 template <typename... KArgs>
 int launch_behind(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t s, const SharedArgs& a) {
@@ -1030,7 +1098,15 @@ int launch_tc(const SharedArgs& a, int* status, cudaStream_t s) {
     return MG_OK;
 }
 
-constexpr int TC_LEAST_PAIRS = 64, TC_CTA_KEYS = 1000;
+template <typename T, bool VEC>
+int launch_simt(const SharedArgs& a, int pairs, cudaStream_t s) {
+    const int nq = simt_pairs(pairs);
+    const size_t smem = sizeof(float) * ((size_t)a.D * nq + (size_t)BLOCK_KEYS * (2 * a.D + 1 + nq));
+    return nq == 8 ? launch_ranges(attention_shared_simt_kernel<T, 8, VEC>, SIMT_THREADS, smem, a, s)
+                   : launch_ranges(attention_shared_simt_kernel<T, 16, VEC>, SIMT_THREADS, smem, a, s);
+}
+
+constexpr int DIRECT_KEYS = 256, TC_LEAST_PAIRS = 64, TC_CTA_KEYS = 1000;
 
 template <int DP>
 int launch_mma(const SharedArgs& a, int pair_tiles, cudaStream_t s) {
@@ -1050,15 +1126,21 @@ size_t sums_at(size_t slots, int head_dim) { return (slots * head_dim + 3) / 4 *
 
 // How a launch is cut.
 struct Cut {
+    bool direct;         // a range a row, no groups: one launch
     bool mma, tc;        // the warp-level tensor cores; shared ranges on tcgen05
     int pair_tiles;      // mma: tiles of 8 pairs that a CTA takes at once
     int row_tiles;       // CTAs that share the pairs of a group
     int shared_slots, own_slots;      // ranges of shared keys, and of a row's own
     int shared_least;
+    int pairs;           // most pairs that a CTA's rows have
+    int launches() const { return direct ? 1 : tc ? 3 : 2; }
 };
 Cut cut(int n_groups, int max_rows, int max_tokens, int max_behind, int n, int n_head, int n_kv_head, int head_dim, int page_tokens,
         bool is_bf16) {
     Cut c;
+    // So few keys that reading them once a row costs less than a second kernel.
+    c.direct = (n_groups == 0 ? max_behind : max_tokens + max_behind) <= DIRECT_KEYS;
+    if (c.direct) n_groups = 0;
     const int share = n_head / n_kv_head, pairs = n_groups > 0 ? (max_rows < n ? max_rows : n) * share : share;
     c.mma = is_bf16 && head_dim % 8 == 0;
     c.tc = n_groups > 0 && is_bf16 && (head_dim == 64 || head_dim == 128) && pairs >= TC_LEAST_PAIRS && page_tokens % 8 == 0 &&
@@ -1066,7 +1148,7 @@ Cut cut(int n_groups, int max_rows, int max_tokens, int max_behind, int n, int n
     const int most_tiles = head_dim <= 64 ? 4 : head_dim <= 128 ? 2 : 1;      // what the registers hold
     const int mma_pairs = c.tc ? share : pairs;
     c.pair_tiles = mma_pairs <= 8 ? 1 : mma_pairs <= 16 && most_tiles > 1 ? 2 : most_tiles;
-    c.row_tiles = ceil_div(pairs, c.tc ? TC_TILES * TC_PAIRS : c.mma ? 8 * c.pair_tiles : SIMT_QUERIES);
+    c.row_tiles = ceil_div(pairs, c.tc ? TC_TILES * TC_PAIRS : c.mma ? 8 * c.pair_tiles : simt_pairs(pairs));
     c.shared_least = c.tc ? TC_KEYS : BLOCK_KEYS;
     const long long shared_ctas = (long long)n_groups * c.row_tiles * n_kv_head, own_ctas = (long long)n * n_kv_head;
     const int most_shared = ceil_div(max_tokens > 0 ? max_tokens : 1, c.shared_least), most_own = ceil_div(max_behind, OWN_LEAST);
@@ -1083,7 +1165,8 @@ Cut cut(int n_groups, int max_rows, int max_tokens, int max_behind, int n, int n
     }
     const long long y = (want + own_ctas - 1) / own_ctas;
     c.shared_slots = (int)(x < 1 ? 1 : x > most_shared ? most_shared : x);
-    c.own_slots = (int)(y < 1 ? 1 : y > most_own ? most_own : y);
+    c.own_slots = c.direct ? 1 : (int)(y < 1 ? 1 : y > most_own ? most_own : y);
+    c.pairs = pairs;
     return c;
 }
 
@@ -1094,6 +1177,7 @@ MG_API long long mg_attention_shared_scratch_floats(int n_groups, int max_rows, 
                                                     int n_kv_head, int head_dim, int page_tokens, int is_bf16) {
     if (n_groups < 0 || max_rows <= 0 || n <= 0 || n_head <= 0 || n_kv_head <= 0 || n_head % n_kv_head != 0 || max_behind <= 0 || page_tokens <= 0) return 0;
     const Cut c = cut(n_groups, max_rows, max_tokens, max_behind, n, n_head, n_kv_head, head_dim, page_tokens, is_bf16 != 0);
+    if (c.direct) return 0;
     const size_t slots = (size_t)n * n_head * (c.shared_slots + c.own_slots);
     return (long long)(sums_at(slots, head_dim) + 2 * slots + n);
 }
@@ -1101,7 +1185,7 @@ MG_API long long mg_attention_shared_scratch_floats(int n_groups, int max_rows, 
 MG_API int mg_attention_shared_launches(int n_groups, int max_rows, int max_tokens, int max_behind, int n, int n_head, int n_kv_head,
                                         int head_dim, int page_tokens, int is_bf16) {
     if (n <= 0 || max_rows <= 0 || n_kv_head <= 0 || n_head % n_kv_head != 0 || max_behind <= 0 || page_tokens <= 0) return 0;
-    return cut(n_groups, max_rows, max_tokens, max_behind, n, n_head, n_kv_head, head_dim, page_tokens, is_bf16 != 0).tc ? 3 : 2;
+    return cut(n_groups, max_rows, max_tokens, max_behind, n, n_head, n_kv_head, head_dim, page_tokens, is_bf16 != 0).launches();
 }
 
 // Attention of n single query tokens, groups of which share their first keys.  q: rows of q_stride elements whose first
@@ -1124,7 +1208,7 @@ MG_API int mg_attention_shared(const void* q, long long q_stride, const void* k_
     MG_REQUIRE(n_head % n_kv_head == 0, "attention: n_head %d is not a multiple of n_kv_head %d", n_head, n_kv_head);
     MG_REQUIRE(n_groups >= 0 && (n_groups == 0 || (groups && max_rows > 0 && max_tokens >= 0)) && max_behind > 0,
                "attention (shared): bad groups or bounds");
-    MG_REQUIRE(scratch != nullptr && q_stride >= (long long)n_head * head_dim, "attention (shared): no scratch, or rows too narrow");
+    MG_REQUIRE(q_stride >= (long long)n_head * head_dim, "attention (shared): rows too narrow");
     MG_REQUIRE((long long)num_pages * n_kv_head * page_tokens < (1ll << 31), "attention (shared): the pool has too many rows");
     if (head_dim > 256 || n_kv_head > 65535)
         return mg_set_error(MG_ERR_UNSUPPORTED, "attention (shared): head_dim %d is more than 256", head_dim);
@@ -1134,6 +1218,9 @@ MG_API int mg_attention_shared(const void* q, long long q_stride, const void* k_
     a.positions = positions; a.groups = groups; a.out = out;
     a.n_groups = n_groups; a.n = n; a.n_head = n_head; a.n_kv_head = n_kv_head; a.D = head_dim; a.page_tokens = page_tokens;
     a.max_pages = max_pages; a.num_pages = num_pages; a.n_requests = n_requests;
+    MG_REQUIRE(c.direct || scratch != nullptr, "attention (shared): no scratch");
+    if (c.direct) a.n_groups = n_groups = 0;
+    a.direct = c.direct; a.element = is_bf16 ? 2 : 4;
     a.first_item = 0; a.shared_least = c.shared_least;
     a.row_tiles = c.row_tiles; a.shared_slots = c.shared_slots; a.own_slots = c.own_slots;
     a.scale_log2e = scale * 1.4426950408889634f;
@@ -1160,10 +1247,10 @@ MG_API int mg_attention_shared(const void* q, long long q_stride, const void* k_
             default: rc = launch_mma<256>(a, c.pair_tiles, s);
         }
     } else {
-        const size_t smem = sizeof(float) * ((size_t)head_dim * SIMT_QUERIES + (size_t)BLOCK_KEYS * (head_dim + 1) + BLOCK_KEYS * SIMT_QUERIES);
-        rc = is_bf16 ? launch_ranges(attention_shared_simt_kernel<bf16>, SIMT_THREADS, smem, a, s)
-                     : launch_ranges(attention_shared_simt_kernel<float>, SIMT_THREADS, smem, a, s);
+        rc = is_bf16 ? launch_simt<bf16, false>(a, c.pairs, s)
+             : head_dim % 4 == 0 && ((((uintptr_t)k_pages | (uintptr_t)v_pages) & 15) == 0) ? launch_simt<float, true>(a, c.pairs, s)
+                                                                                           : launch_simt<float, false>(a, c.pairs, s);
     }
-    if (rc != MG_OK) return rc;
+    if (rc != MG_OK || c.direct) return rc;
     return is_bf16 ? launch_join<bf16>(a, s) : launch_join<float>(a, s);
 }

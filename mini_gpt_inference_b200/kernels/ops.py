@@ -990,7 +990,7 @@ class CudaOps:
         sizes = (groups.shape[0], int(shared.max_rows), int(shared.max_tokens), int(shared.max_behind))
         shape = (*sizes, n, n_head, n_kv_head, head_dim, cache.page_tokens, is_bf16)
         floats = self.lib.mg_attention_shared_scratch_floats(*shape)
-        scratch = torch.empty((floats,), dtype=torch.float32, device=self.device)
+        scratch = torch.empty((floats,), dtype=torch.float32, device=self.device) if floats else None      # (few keys: one kernel)
         self._run(self.lib.mg_attention_shared(
             _ptr(qkv), qkv.shape[1], _ptr(k), _ptr(v), _ptr(table), _ptr(ctx.token_request), _ptr(ctx.positions), _ptr(groups),
             *sizes, _ptr(out), _ptr(scratch), n, n_head, n_kv_head, head_dim, cache.page_tokens, table.shape[1], k.shape[0],
