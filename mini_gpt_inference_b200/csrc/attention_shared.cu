@@ -1152,7 +1152,8 @@ Cut cut(int n_groups, int max_rows, int max_tokens, int max_behind, int n, int n
     c.shared_least = c.tc ? TC_KEYS : BLOCK_KEYS;
     const long long shared_ctas = (long long)n_groups * c.row_tiles * n_kv_head, own_ctas = (long long)n * n_kv_head;
     const int most_shared = ceil_div(max_tokens > 0 ? max_tokens : 1, c.shared_least), most_own = ceil_div(max_behind, OWN_LEAST);
-    const long long want = 148 * 4;
+    // (CTAs of each kind; 8 x 8 rows of about 1,021 shared tokens, 8 heads of 64: 14.2 us with two an SM, 16.9 with four, 15.3 with one)
+    const long long want = 148 * 2;
     long long x = shared_ctas > 0 ? (want + shared_ctas - 1) / shared_ctas : 1;
     if (c.tc) {
         // one CTA an SM: the number of ranges whose rounds of CTAs take the fewest keys, what a CTA costs besides its keys
