@@ -56,6 +56,11 @@ class RequestCache:
     serial: int = 0
     version: int = 0
     capacity: int = 0                                 # tokens its pages have room for (every group)
+    # A request that was forked off another holds that one's full pages too, per group its first `shared` ones; they belong
+    # to the other (its `parent`), which has `forks` such requests and cannot be released before them.
+    shared: list[int] = field(default_factory=list)
+    parent: str | None = None
+    forks: int = 0
 
 
 class CacheManager:
@@ -173,8 +178,25 @@ class CacheManager:
             raise CacheFullError("no state slot free")
         self._serial += 1
         req = RequestCache(request_id, self.slots.take_one(), 0, [[] for _ in self.groups], self._serial,
-                           capacity=0 if self.groups else 1 << 30)
+                           capacity=0 if self.groups else 1 << 30, shared=[0] * len(self.groups))
         self.requests[request_id] = req
+        return req
+
+    def fork(self, request_id: str, parent_id: str) -> RequestCache:
+        """Admit a request that goes on from where another is: the pages that the other has filled are in its tables too (and
+        stay the other's), the part-filled page and what comes behind it are taken by ``reserve``.  What a page or a state
+        slot holds is the caller's to copy."""
+        parent = self.get(parent_id)
+        if parent.parent is not None:
+            raise PoolError(f"request {parent_id!r} is a fork itself")
+        req = self.admit(request_id)
+        for g, group in enumerate(self.groups):
+            req.shared[g] = parent.length // group.page_tokens
+            req.tables[g] = parent.tables[g][: req.shared[g]]
+        req.parent, req.length = parent_id, parent.length
+        parent.forks += 1
+        req.capacity = (min(len(t) * group.page_tokens for t, group in zip(req.tables, self.groups))
+                        if req.tables else 1 << 30)
         return req
 
     def has(self, request_id: str) -> bool:
@@ -235,12 +257,12 @@ class CacheManager:
         if new_length > req.capacity:
             raise PoolError(f"request {request_id!r} advanced past its reserved pages")
         req.length = new_length
-        if not self._any_window:
+        if not self._any_window or req.forks:             # (pages that forks read stay)
             return
         for g, group in enumerate(self.groups):
             first = self._first_live_page(group, new_length)
             table = req.tables[g]
-            kept = self._kept_pages(group.spec, group.page_tokens)
+            kept = max(self._kept_pages(group.spec, group.page_tokens), req.shared[g])
             passed = [p for p in table[kept:first] if p != NO_PAGE]
             if passed:
                 group.pool.give_back(passed)
@@ -250,8 +272,12 @@ class CacheManager:
 
     def release(self, request_id: str) -> None:
         req = self.get(request_id)
+        if req.forks:
+            raise PoolError(f"request {request_id!r} has {req.forks} forks that hold its pages")
+        if req.parent is not None:
+            self.get(req.parent).forks -= 1
         for g, group in enumerate(self.groups):
-            group.pool.give_back([p for p in req.tables[g] if p != NO_PAGE])
+            group.pool.give_back([p for p in req.tables[g][req.shared[g]:] if p != NO_PAGE])
             req.tables[g] = []
         self.slots.give_back([req.state_slot])
         del self.requests[request_id]
@@ -277,7 +303,10 @@ class CacheManager:
         held_tokens = used_tokens = 0
         for r in self.requests.values():
             for g, group in enumerate(self.groups):
-                held_tokens += sum(1 for p in r.tables[g] if p != NO_PAGE) * group.page_tokens
+                held_tokens += sum(1 for p in r.tables[g][r.shared[g]:] if p != NO_PAGE) * group.page_tokens
+                if r.parent is not None:                  # (the shared pages are counted with the request they belong to)
+                    used_tokens += r.length - r.shared[g] * group.page_tokens
+                    continue
                 first = self._first_live_page(group, r.length) * group.page_tokens
                 kept = min(first, self._kept_pages(group.spec, group.page_tokens) * group.page_tokens)
                 used_tokens += max(0, r.length - first) + min(kept, r.length)
@@ -290,12 +319,15 @@ class CacheManager:
         }
 
     def check(self) -> None:
-        """Every page is either free or in exactly one table; the same for slots."""
+        """Every page is either free or in exactly one table (those of forks aside, which hold their parent's too); the same for
+        slots."""
         for g, group in enumerate(self.groups):
             group.pool.check()
             seen: set[int] = set()
             for r in self.requests.values():
-                for p in r.tables[g]:
+                if r.tables[g][: r.shared[g]] != (self.get(r.parent).tables[g][: r.shared[g]] if r.parent is not None else []):
+                    raise PoolError(f"request {r.request_id!r} shares pages that its parent does not have")
+                for p in r.tables[g][r.shared[g]:]:
                     if p == NO_PAGE:
                         continue
                     if p in seen:

@@ -30,6 +30,9 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--top-k", type=int, default=50)
     ap.add_argument("--top-p", type=float, default=None)
     ap.add_argument("--seed", type=int, default=None)
+    ap.add_argument("--beams", type=int, default=None, help="search for the best continuations with so many beams, in place of sampling")
+    ap.add_argument("--length-penalty", type=float, default=0.0, help="with --beams: rank by the log probability over length to this power")
+    ap.add_argument("--eot-id", type=int, default=None, help="with --beams: the token id that ends a continuation")
     ap.add_argument("--vocab-limit", type=int, default=None,
                     help="ids at and above this are never sampled: rows that only pad the embedding "
                          "table (the reference masks ids >= 50257 of its 50304 rows)")
@@ -82,7 +85,7 @@ def main(argv=None) -> int:
     else:
         raise SystemExit("give --prompt-ids or --prompt")
 
-    from . import EngineConfig, LLMEngine, SamplingParams
+    from . import BeamParams, EngineConfig, LLMEngine, SamplingParams
 
     engine = LLMEngine.from_pretrained(args.model, EngineConfig(
         block_size=args.kv_block_size, num_blocks=args.num_kv_blocks,
@@ -90,6 +93,10 @@ def main(argv=None) -> int:
         dtype=args.dtype, device=args.device), vocab_limit=args.vocab_limit)
     print(f"config: {engine.config}", file=sys.stderr)
     print(f"params: {engine.config.num_parameters() / 1e6:.1f}M", file=sys.stderr)
+    if args.beams is not None:
+        found = engine.beam_search([prompt], BeamParams(args.beams, args.max_new_tokens, args.length_penalty), args.eot_id)[0]
+        print(json.dumps({"prompt_ids": prompt, "beams": found}))
+        return 0
     params = SamplingParams(max_tokens=args.max_new_tokens, temperature=args.temperature,
                             top_k=args.top_k, top_p=args.top_p, seed=args.seed)
     out = engine.generate([prompt], params)[0]

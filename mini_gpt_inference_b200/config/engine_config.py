@@ -12,6 +12,7 @@ unlike the reference, ``seed`` is honoured (per-request counter-based RNG).
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass, field
 
 
@@ -51,6 +52,24 @@ def canonical_dtype(name: str) -> str:
     if key not in table:
         raise ValueError(f"dtype must be bfloat16 or float32, got {name!r}")
     return table[key]
+
+
+@dataclass
+class BeamParams:
+    """A beam search: the ``beams`` best continuations at every step, ranked by the sum of their tokens' log probabilities over
+    ``length ** length_penalty``."""
+
+    beams: int = 4
+    max_tokens: int = 128
+    length_penalty: float = 0.0
+
+    def __post_init__(self) -> None:
+        if not 1 <= self.beams <= 32:
+            raise ValueError("beams must be 1 to 32")
+        if self.max_tokens <= 0:
+            raise ValueError("max_tokens must be positive")
+        if not math.isfinite(self.length_penalty):
+            raise ValueError("length_penalty must be a finite number")
 
 
 @dataclass

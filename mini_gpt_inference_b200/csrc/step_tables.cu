@@ -31,6 +31,7 @@ struct TableArgs {
     int* token_request;
     int* positions;
     int* q_start;
+    int* after;
     int n_requests, n_tokens, pool_rows, n_groups;
     TableGroup group[MAX_GROUPS];
 };
@@ -57,7 +58,10 @@ __global__ void __launch_bounds__(THREADS) step_tables_kernel(const __grid_const
     for (int w = 0; w < warp; ++w) at += warp_total[w];
     for (int r = r0; r < r1; ++r) {
         starts[r] = at;
-        if (blockIdx.x == 0) a.q_start[r] = at;
+        if (blockIdx.x == 0) {
+            a.q_start[r] = at;
+            a.after[r] = a.before[r] + max(0, a.fresh[r]);
+        }
         at += max(0, a.fresh[r]);
     }
     if (tid == THREADS - 1) starts[a.n_requests] = at;
@@ -110,13 +114,14 @@ __global__ void __launch_bounds__(THREADS) step_tables_kernel(const __grid_const
 // addresses of its pages [pool_rows, width] (below zero: none), of the block tables [n_requests, width] and of the cache rows
 // [n_tokens] to be written, width, and tokens of a page.  Token rows behind the last request's are padding: position and cache
 // row -1, request 0.  A number of new tokens below zero counts as none.
+// after: [n_requests], before + fresh.
 MG_API int mg_step_tables(const int* rows, const int* before, const int* fresh, int* token_request, int* positions, int* q_start,
-                          int n_requests, int n_tokens, int pool_rows, int n_groups, const long long* groups, void* stream) {
+                          int* after, int n_requests, int n_tokens, int pool_rows, int n_groups, const long long* groups, void* stream) {
     if (n_requests == 0 && n_tokens == 0) return MG_OK;
     MG_REQUIRE(n_requests > 0 && n_tokens >= 0 && pool_rows > 0 && n_groups >= 0, "step_tables: bad sizes");
     MG_REQUIRE(n_requests <= MAX_REQUESTS && n_groups <= MAX_GROUPS, "step_tables: at most %d requests and %d groups", MAX_REQUESTS, MAX_GROUPS);
     TableArgs a = {};
-    a.rows = rows; a.before = before; a.fresh = fresh; a.token_request = token_request; a.positions = positions; a.q_start = q_start;
+    a.rows = rows; a.before = before; a.fresh = fresh; a.token_request = token_request; a.positions = positions; a.q_start = q_start; a.after = after;
     a.n_requests = n_requests; a.n_tokens = n_tokens; a.pool_rows = pool_rows; a.n_groups = n_groups;
     for (int g = 0; g < n_groups; ++g) {
         const long long* z = groups + 5 * g;

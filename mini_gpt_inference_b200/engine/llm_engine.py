@@ -22,8 +22,9 @@ from typing import Any, Sequence
 
 import torch
 
-from ..config.engine_config import EngineConfig, SamplingParams
+from ..config.engine_config import BeamParams, EngineConfig, SamplingParams
 from ..sampling.sampler import Sampler
+from .beam_search import BeamSearch
 from .build import LoadedModel, load_model, make_runner
 from .request import Request, RequestOutput, SequenceState
 from .runner import ModelRunner, StepEntry
@@ -65,6 +66,7 @@ class LLMEngine:
         self.runner.greedy_vocab_limit = vocab_limit     # before the first decode step is captured
         self.max_context = self.runner.max_context
         self._sequences: dict[str, SequenceState] = {}
+        self._beam_search: BeamSearch | None = None
         # Steady decoding overlaps the host with the device: a step is launched with the tokens
         # of the step before still on the device, and that step's ids are read while this one
         # runs.  What step() returns then lags one step behind what the device has computed.
@@ -98,22 +100,11 @@ class LLMEngine:
         return {"decode_graphs_captured": made}
 
     def add_request(self, request: Request) -> None:
-        prompt_len = len(request.prompt_token_ids)
-        if prompt_len == 0:
+        if len(request.prompt_token_ids) == 0:
             raise ValueError(f"request {request.request_id!r} has an empty prompt")
         if request.request_id in self._sequences:
             raise ValueError(f"request id {request.request_id!r} is already in use")
-        vocab = self.runner.vocab_size
-        bad = [t for t in request.prompt_token_ids if not (0 <= t < vocab)]
-        if bad:
-            raise ValueError(f"request {request.request_id!r}: token id {bad[0]} is outside the "
-                             f"vocabulary (0..{vocab - 1})")
-        longest = prompt_len + request.sampling_params.max_tokens
-        if longest > self.max_context:
-            raise ValueError(
-                f"prompt_len ({prompt_len}) + max_tokens ({request.sampling_params.max_tokens}) "
-                f"= {longest} > {self.max_context}; this request can never finish without "
-                "running past the position table")
+        self._check_prompt(f"request {request.request_id!r}", request.prompt_token_ids, request.sampling_params.max_tokens)
         if request.sampling_params.stop and self.token_bytes is None:
             raise ValueError(
                 f"request {request.request_id!r} sets stop strings, but the engine was given no "
@@ -126,6 +117,19 @@ class LLMEngine:
                             seed=self.sampler.fresh_seed() if seed is None else int(seed))
         self.scheduler.add_request(seq)
         self._sequences[request.request_id] = seq
+
+    def _check_prompt(self, whose: str, prompt, max_tokens: int) -> None:
+        vocab = self.runner.vocab_size
+        bad = [t for t in prompt if not (0 <= t < vocab)]
+        if bad:
+            raise ValueError(f"{whose}: token id {bad[0]} is outside the "
+                             f"vocabulary (0..{vocab - 1})")
+        longest = len(prompt) + max_tokens
+        if longest > self.max_context:
+            raise ValueError(
+                f"prompt_len ({len(prompt)}) + max_tokens ({max_tokens}) "
+                f"= {longest} > {self.max_context}; this request can never finish without "
+                "running past the position table")
 
     def has_unfinished_requests(self) -> bool:
         return self.scheduler.has_work() or self._inflight is not None or bool(self._held_outputs)
@@ -311,6 +315,31 @@ class LLMEngine:
                     if out.finished:
                         results[out.request_id]["finish_reason"] = out.finish_reason
         return [results[rid] for rid in ids]
+
+    def beam_search(self, prompts: Sequence[Sequence[int]], params: BeamParams | None = None,
+                    eot_token_id: int | None = None) -> list[list[dict]]:
+        """The best continuations of every prompt (``BeamParams``).  All prompts' beams run as one batch, step after step on
+        the device; requests that the engine holds wait meanwhile and keep their caches.  Returns, in the order of the prompts,
+        up to ``beams`` dicts, the best first, with ``token_ids`` (generated only, an end of text included), ``logprob`` (the sum
+        of their log probabilities), ``score`` (what they are ranked by) and ``finish_reason`` (``"eot"`` or ``"length"``).
+        Raises ``CacheFullError`` where the pools do not hold ``beams`` requests per prompt (beams share their prompt's pages)."""
+        params = params or BeamParams()
+        for i, prompt in enumerate(prompts):
+            if len(prompt) == 0:
+                raise ValueError(f"prompt {i} is empty")
+            self._check_prompt(f"prompt {i}", prompt, params.max_tokens)
+        limit = self.sampler.vocab_limit or self.runner.vocab_size
+        if params.beams > limit:
+            raise ValueError(f"{params.beams} beams of {limit} token ids")
+        if eot_token_id is not None and not 0 <= eot_token_id < limit:
+            raise ValueError(f"eot_token_id {eot_token_id} is not among the {limit} token ids that can be generated")
+        if not prompts:
+            return []
+        # What is still on its way from the device is read first: its ids lie where the prompts' steps leave theirs.
+        self._held_outputs.extend(self._drain())
+        if self._beam_search is None:
+            self._beam_search = BeamSearch(self.runner, self.engine_cfg.prefill_chunk)
+        return self._beam_search.run([list(p) for p in prompts], params, eot_token_id, self.sampler.vocab_limit)
 
     def stats(self) -> dict:
         out = dict(self.runner.manager.stats())

@@ -107,7 +107,7 @@ _SIGNATURES = {
     "mg_attention_shared_launches": [_I] * 10,
     "mg_beam_select": [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, ctypes.c_double, _P, _P, _P, _P, _P, _P, _P, _P],
     "mg_beam_reorder": [_P, _P, _P, _I, _I, _I, _P, _P, _P],
-    "mg_step_tables": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P],
+    "mg_step_tables": [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P],
     "mg_copy_ints": [_P, _P, _I, _P],
     "mg_argmax": [_P, _P, _I, _I, _I, _P],
     "mg_argmax_wide": [_P, _P, _P, _P, _I, _I, _I, _P],

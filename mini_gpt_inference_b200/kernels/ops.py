@@ -23,6 +23,7 @@ EPILOGUES = {"none": 0, "gelu_tanh": 1, "residual": 2, "relu_sq": 3}
 PLAIN_ACTIVATIONS = {"relu_sq": 0, "gelu_tanh": 1, "silu": 2}           # ... and the activation of a unit without a gate
 GATED_ACTIVATIONS = {"silu": 0, "clamped_swish": 1, "gelu_tanh": 2}     # the gated product of a unit's two halves
 MAX_BEAMS = 32           # most beams of a group in a search
+REORDER_GROUPS, REORDER_STATES = 8, 48      # most cache groups and state tensors of one launch that hands caches over
 MOE_TC_EXPERTS = 256     # most experts the tensor-core tiles take
 MOE_FEW_TOKENS = 16      # most tokens the experts' kernels for few tokens take
 # More tokens than this take the heads' small products on the tensor-core GEMM.  (us, mma.sync / tcgen05: 16 heads of 128 -> 512
@@ -101,6 +102,7 @@ class StepTables:
     req_q_start: torch.Tensor
     block_tables: list
     slot_mapping: list
+    ctx_after: torch.Tensor               # [R] tokens in the cache once the step's are in
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
@@ -1927,9 +1929,12 @@ class CudaOps:
                 kept += (state.data_ptr(), state.numel() // state.shape[0] * state.element_size(), state.shape[0])
         if rows == 0 or not (paged or kept):
             return
-        self._run(self.lib.mg_beam_reorder(
-            _ptr(parents), _ptr(lengths), _ptr(slots), rows, len(paged) // 10, len(kept) // 3, _numbers(paged), _numbers(kept),
-            self._stream()), "beam_reorder")
+        while paged or kept:                                     # (a launch takes so many of each)
+            now, paged = paged[: 10 * REORDER_GROUPS], paged[10 * REORDER_GROUPS:]
+            also, kept = kept[: 3 * REORDER_STATES], kept[3 * REORDER_STATES:]
+            self._run(self.lib.mg_beam_reorder(
+                _ptr(parents), _ptr(lengths), _ptr(slots), rows, len(now) // 10, len(also) // 3, _numbers(now), _numbers(also),
+                self._stream()), "beam_reorder")
 
     def step_tables(self, pages, page_tokens, ctx_before, q_len, num_tokens, rows=None):
         """A step's integers from the lengths of its requests, on the device: request ``r`` has ``ctx_before[r]`` tokens in
@@ -1955,15 +1960,16 @@ class CudaOps:
             raise KernelLibraryError("step_tables: fewer rows of pages than requests")
         if R == 0:
             raise KernelLibraryError("step_tables: no requests")
-        parts = [n] * (2 + groups) + [R] + [R * width for width in widths]
+        parts = [n] * (2 + groups) + [R, R] + [R * width for width in widths]
         parts = torch.empty((sum(parts),), dtype=torch.int32, device=self.device).split(parts)
-        out = StepTables(parts[0], parts[1], parts[2 + groups], [t.view(R, width) for t, width in zip(parts[3 + groups:], widths)],
-                         list(parts[2: 2 + groups]))
+        out = StepTables(parts[0], parts[1], parts[2 + groups], [t.view(R, width) for t, width in zip(parts[4 + groups:], widths)],
+                         list(parts[2: 2 + groups]), parts[3 + groups])
         numbers = []
         for pool, table, slots, width, size in zip(pages, out.block_tables, out.slot_mapping, widths, page_tokens):
             numbers += (pool.data_ptr(), table.data_ptr(), slots.data_ptr(), width, int(size))
         self._run(self.lib.mg_step_tables(
-            _ptr(rows), _ptr(ctx_before), _ptr(q_len), _ptr(out.token_request), _ptr(out.positions), _ptr(out.req_q_start), R, n,
+            _ptr(rows), _ptr(ctx_before), _ptr(q_len), _ptr(out.token_request), _ptr(out.positions), _ptr(out.req_q_start), _ptr(out.ctx_after),
+            R, n,
             pool_rows, groups, _numbers(numbers), self._stream()), "step_tables")
         return out
 

@@ -99,3 +99,24 @@ def step_tables(pages, page_tokens, ctx_before, q_len, num_tokens, rows=None):
     real = min(len(request), num_tokens)
     pad = num_tokens - real
     return (request[:real] + [0] * pad, positions[:real] + [-1] * pad, start, tables, [s[:real] + [-1] * pad for s in slots])
+
+
+def search(last_logits, prompt, beams, max_tokens, length_penalty=0.0, end_token=None, vocab_limit=None):
+    """Beam search one hypothesis at a time: ``last_logits(tokens)`` gives the logits behind them.  Best first:
+    ``(tokens, log probability, ended)``."""
+    made = [([], 0.0, False)]
+    for _ in range(max_tokens):
+        candidates = []
+        for ids, score, over in made:
+            if over:
+                candidates.append((ids, score, True))
+                continue
+            x = last_logits(list(prompt) + ids).double()
+            x = torch.log_softmax(x[: vocab_limit or x.numel()], -1)
+            for t in torch.topk(x, min(beams, x.numel())).indices.tolist():
+                candidates.append((ids + [t], score + float(x[t]), t == end_token))
+        candidates.sort(key=lambda c: -c[1] / len(c[0]) ** length_penalty)
+        made = candidates[:beams]
+        if all(over for _, _, over in made):
+            break
+    return made
