@@ -55,6 +55,19 @@ __device__ __forceinline__ int range_keys(int keys, int slots, int least) {
 
 constexpr int OWN_LEAST = 64;
 
+// A group's shared tokens: a number that no row's block table reaches (or below zero) counts as none.
+__device__ __forceinline__ int tokens_of(const SharedArgs& a, int group) {
+    const int tokens = a.groups[3 * group + 2];
+    return tokens < 0 || tokens > (long long)a.max_pages * a.page_tokens ? 0 : tokens;
+}
+
+// A row's position, at most the last that its block table reaches; below zero: padding.
+__device__ __forceinline__ int position_of(const SharedArgs& a, int row) {
+    const int p = a.positions[row];
+    const long long last = (long long)a.max_pages * a.page_tokens - 1;
+    return p > last ? (int)last : p;
+}
+
 // The shared tokens of the group that `row` belongs to (0: none); every warp finds them for itself.
 __device__ __forceinline__ int group_tokens(const SharedArgs& a, int row) {
     const int lane = threadIdx.x & 31;
@@ -65,8 +78,8 @@ __device__ __forceinline__ int group_tokens(const SharedArgs& a, int row) {
         int shared = 0;
         if (g < a.n_groups) {
             const int first = a.groups[3 * g], rows = a.groups[3 * g + 1];
-            shared = a.groups[3 * g + 2];
-            mine = row >= first && row - first < rows;
+            shared = tokens_of(a, g);
+            mine = first >= 0 && row >= first && row - first < rows;
         }
         const uint32_t found = __ballot_sync(0xffffffffu, mine);
         if (found) tokens = __shfl_sync(0xffffffffu, shared, __ffs(found) - 1);
@@ -97,7 +110,7 @@ __device__ __forceinline__ bool item_of(const SharedArgs& a, int item, Item& it)
         const int g = item / a.row_tiles;
         it.first_row = a.groups[3 * g];
         it.rows = a.groups[3 * g + 1];
-        it.shared_keys = a.groups[3 * g + 2];
+        it.shared_keys = tokens_of(a, g);
         if (it.first_row < 0 || it.rows <= 0 || it.first_row >= a.n) return false;
         it.rows = min(it.rows, a.n - it.first_row);
         request = a.token_request[it.first_row];
@@ -108,7 +121,7 @@ __device__ __forceinline__ bool item_of(const SharedArgs& a, int item, Item& it)
         item -= shared_items;
         it.slot = item % a.own_slots;
         it.first_row = item / a.own_slots;
-        const int p = a.positions[it.first_row];
+        const int p = position_of(a, it.first_row);
         request = a.token_request[it.first_row];
         int behind = group_tokens(a, it.first_row);
         if (behind > p + 1) behind = 0;
@@ -145,7 +158,7 @@ __device__ __forceinline__ int cache_row(const SharedArgs& a, const Item& it, in
 __device__ __forceinline__ int pair_row(const SharedArgs& a, const Item& it, int j, int share) {
     if (j >= it.rows * share) return -1;
     const int row = it.first_row + j / share;
-    return !it.shared || a.positions[row] + 1 >= it.shared_keys ? row : -1;
+    return !it.shared || position_of(a, row) + 1 >= it.shared_keys ? row : -1;
 }
 
 // What a range leaves of feature d of a (row, head): the unnormalised average, with the maximum and the sum, or, where a row has one
@@ -990,7 +1003,7 @@ template <typename T, int J>
 __global__ void __launch_bounds__(128) attention_shared_join_kernel(SharedArgs a) {
     const int row = blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (head >= a.n_head) return;
-    const int p = a.positions[row];
+    const int p = position_of(a, row);
     T* const out = (T*)a.out + ((size_t)row * a.n_head + head) * a.D;
     pdl_wait();
     pdl_trigger();
@@ -1125,6 +1138,7 @@ int padded_head(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 2
 size_t sums_at(size_t slots, int head_dim) { return (slots * head_dim + 3) / 4 * 4; }
 
 // How a launch is cut.
+enum Kind { F32 = 0, BF16_ALIGNED = 1, BF16 = 2 };      // aligned: pages and rows of queries at 16-byte boundaries
 struct Cut {
     bool direct;         // a range a row, no groups: one launch
     bool mma, tc;        // the warp-level tensor cores; shared ranges on tcgen05
@@ -1136,14 +1150,14 @@ struct Cut {
     int launches() const { return direct ? 1 : tc ? 3 : 2; }
 };
 Cut cut(int n_groups, int max_rows, int max_tokens, int max_behind, int n, int n_head, int n_kv_head, int head_dim, int page_tokens,
-        bool is_bf16) {
+        int kind) {
     Cut c;
     // So few keys that reading them once a row costs less than a second kernel.
     c.direct = (n_groups == 0 ? max_behind : max_tokens + max_behind) <= DIRECT_KEYS;
     if (c.direct) n_groups = 0;
     const int share = n_head / n_kv_head, pairs = n_groups > 0 ? (max_rows < n ? max_rows : n) * share : share;
-    c.mma = is_bf16 && head_dim % 8 == 0;
-    c.tc = n_groups > 0 && is_bf16 && (head_dim == 64 || head_dim == 128) && pairs >= TC_LEAST_PAIRS && page_tokens % 8 == 0 &&
+    c.mma = kind == BF16_ALIGNED && head_dim % 8 == 0;
+    c.tc = n_groups > 0 && kind == BF16_ALIGNED && (head_dim == 64 || head_dim == 128) && pairs >= TC_LEAST_PAIRS && page_tokens % 8 == 0 &&
            (page_tokens < TC_KEYS ? TC_KEYS % page_tokens == 0 : page_tokens % TC_KEYS == 0) && max_tokens >= TC_KEYS;
     const int most_tiles = head_dim <= 64 ? 4 : head_dim <= 128 ? 2 : 1;      // what the registers hold
     const int mma_pairs = c.tc ? share : pairs;
@@ -1175,18 +1189,18 @@ Cut cut(int n_groups, int max_rows, int max_tokens, int max_behind, int n, int n
 
 // Floats of scratch that mg_attention_shared() takes for these sizes and bounds.
 MG_API long long mg_attention_shared_scratch_floats(int n_groups, int max_rows, int max_tokens, int max_behind, int n, int n_head,
-                                                    int n_kv_head, int head_dim, int page_tokens, int is_bf16) {
+                                                    int n_kv_head, int head_dim, int page_tokens, int kind) {
     if (n_groups < 0 || max_rows <= 0 || n <= 0 || n_head <= 0 || n_kv_head <= 0 || n_head % n_kv_head != 0 || max_behind <= 0 || page_tokens <= 0) return 0;
-    const Cut c = cut(n_groups, max_rows, max_tokens, max_behind, n, n_head, n_kv_head, head_dim, page_tokens, is_bf16 != 0);
+    const Cut c = cut(n_groups, max_rows, max_tokens, max_behind, n, n_head, n_kv_head, head_dim, page_tokens, kind);
     if (c.direct) return 0;
     const size_t slots = (size_t)n * n_head * (c.shared_slots + c.own_slots);
     return (long long)(sums_at(slots, head_dim) + 2 * slots + n);
 }
 
 MG_API int mg_attention_shared_launches(int n_groups, int max_rows, int max_tokens, int max_behind, int n, int n_head, int n_kv_head,
-                                        int head_dim, int page_tokens, int is_bf16) {
+                                        int head_dim, int page_tokens, int kind) {
     if (n <= 0 || max_rows <= 0 || n_kv_head <= 0 || n_head % n_kv_head != 0 || max_behind <= 0 || page_tokens <= 0) return 0;
-    return cut(n_groups, max_rows, max_tokens, max_behind, n, n_head, n_kv_head, head_dim, page_tokens, is_bf16 != 0).launches();
+    return cut(n_groups, max_rows, max_tokens, max_behind, n, n_head, n_kv_head, head_dim, page_tokens, kind).launches();
 }
 
 // Attention of n single query tokens, groups of which share their first keys.  q: rows of q_stride elements whose first
@@ -1196,13 +1210,15 @@ MG_API int mg_attention_shared_launches(int n_groups, int max_rows, int max_toke
 // same keys and values over the shared tokens.  max_rows, max_tokens, max_behind: how many rows a group has, how many
 // tokens it shares and how many keys a row has besides, at most (bounds that are too low cost time).  A row whose position
 // is below zero is padding: its output is zeros.  scratch: mg_attention_shared_scratch_floats() floats, 16-byte aligned,
-// that no other launch uses meanwhile.  status: a word that gets a code if a bounded wait runs out.  mg_attention_shared_launches()
+// that no other launch uses meanwhile.  kind: 0 32-bit, 1 bfloat16 with pages and rows of queries at 16-byte boundaries, 2 other
+// bfloat16.  status: a word that gets a code if a bounded wait runs out.  mg_attention_shared_launches()
 // launches.  MG_ERR_UNSUPPORTED for heads of more than 256 features.
 MG_API int mg_attention_shared(const void* q, long long q_stride, const void* k_pages, const void* v_pages, const int* table,
                                const int* token_request, const int* positions, const int* groups, int n_groups, int max_rows,
                                int max_tokens, int max_behind, void* out, float* scratch, int n, int n_head, int n_kv_head,
                                int head_dim, int page_tokens, int max_pages, int num_pages, int n_requests, float scale,
-                               int is_bf16, int* status, void* stream) {
+                               int kind, int* status, void* stream) {
+    const bool is_bf16 = kind != F32;
     if (n == 0) return MG_OK;
     MG_REQUIRE(n > 0 && n_head > 0 && n_kv_head > 0 && head_dim > 0 && page_tokens > 0 && max_pages > 0 && num_pages > 0 && n_requests > 0,
                "attention (shared): bad sizes");
@@ -1214,7 +1230,7 @@ MG_API int mg_attention_shared(const void* q, long long q_stride, const void* k_
     if (head_dim > 256 || n_kv_head > 65535)
         return mg_set_error(MG_ERR_UNSUPPORTED, "attention (shared): head_dim %d is more than 256", head_dim);
     SharedArgs a;
-    const Cut c = cut(n_groups, max_rows, max_tokens, max_behind, n, n_head, n_kv_head, head_dim, page_tokens, is_bf16 != 0);
+    const Cut c = cut(n_groups, max_rows, max_tokens, max_behind, n, n_head, n_kv_head, head_dim, page_tokens, kind);
     a.q = q; a.q_stride = q_stride; a.k_pages = k_pages; a.v_pages = v_pages; a.table = table; a.token_request = token_request;
     a.positions = positions; a.groups = groups; a.out = out;
     a.n_groups = n_groups; a.n = n; a.n_head = n_head; a.n_kv_head = n_kv_head; a.D = head_dim; a.page_tokens = page_tokens;
@@ -1233,8 +1249,8 @@ MG_API int mg_attention_shared(const void* q, long long q_stride, const void* k_
     MG_REQUIRE(items < (1ll << 31), "attention (shared): too many rows");
     cudaStream_t s = (cudaStream_t)stream;
     int rc;
-    if (c.mma && ((((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages) & 15) || q_stride % 2))
-        return mg_set_error(MG_ERR_ARG, "attention (shared): queries and pages have to be 16-byte aligned, rows of queries 4-byte aligned");
+    MG_REQUIRE(kind != BF16_ALIGNED || (q_stride % 8 == 0 && (((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages) & 15) == 0),
+               "attention (shared): rows that are said to be 16-byte aligned and are not");
     if (c.tc) {
         rc = head_dim == 64 ? launch_tc<64>(a, status, s) : launch_tc<128>(a, status, s);
         if (rc != MG_OK) return rc;

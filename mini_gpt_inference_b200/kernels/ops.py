@@ -968,10 +968,13 @@ class CudaOps:
         keys 0 .. its position of its own request; a row in front of the end of its group's shared tokens, or of no group,
         reads all of them for itself; one at a position below zero is padding, its result zeros.  Heads of up to 256
         features; no window, no values in the key rows."""
-        shared = ctx.shared_prefix
+        shared = getattr(ctx, "shared_prefix", None)
+        if shared is None:
+            raise KernelLibraryError("attention (shared): the step names no groups of rows")
         k, v, n = cache.k_pages, cache.v_pages, qkv.shape[0]
         self._want(qkv, k.dtype, "qkv", 2)
-        is_bf16 = self._is_bf16(qkv)
+        # 32-bit, bfloat16 at 16-byte boundaries, other bfloat16
+        kind = self._is_bf16(qkv) and (2 if qkv.shape[1] % 8 or (qkv.data_ptr() | k.data_ptr() | v.data_ptr()) % 16 else 1)
         table = self._want(ctx.block_tables[cache.group], torch.int32, "block_table", 2)
         groups = self._want(shared.groups, torch.int32, "groups of rows", 2)
         if self._want(v, k.dtype, "v_pages", 4).shape != self._want(k, None, "k_pages", 4).shape or (
@@ -986,17 +989,17 @@ class CudaOps:
             raise KernelLibraryError("attention (shared): one request and one position per row")
         if shared.max_rows < 1 or shared.max_tokens < 0 or shared.max_behind < 1:
             raise KernelLibraryError("attention (shared): bounds below one row or one key")
-        out = torch.empty((n, n_head * head_dim), dtype=qkv.dtype, device=self.device)
+        out = qkv.new_empty((n, n_head * head_dim))
         if n == 0:
             return out
         sizes = (groups.shape[0], int(shared.max_rows), int(shared.max_tokens), int(shared.max_behind))
-        shape = (*sizes, n, n_head, n_kv_head, head_dim, cache.page_tokens, is_bf16)
+        shape = (*sizes, n, n_head, n_kv_head, head_dim, cache.page_tokens, kind)
         floats = self.lib.mg_attention_shared_scratch_floats(*shape)
-        scratch = torch.empty((floats,), dtype=torch.float32, device=self.device) if floats else None      # (few keys: one kernel)
+        scratch = table.new_empty((floats,)) if floats else None         # (words of 32 bits; few keys: one kernel, no scratch)
         self._run(self.lib.mg_attention_shared(
             _ptr(qkv), qkv.shape[1], _ptr(k), _ptr(v), _ptr(table), _ptr(ctx.token_request), _ptr(ctx.positions), _ptr(groups),
             *sizes, _ptr(out), _ptr(scratch), n, n_head, n_kv_head, head_dim, cache.page_tokens, table.shape[1], k.shape[0],
-            table.shape[0], float(scale), is_bf16, _ptr(self.status), self._stream()), "paged_attention (shared)")
+            table.shape[0], float(scale), kind, _ptr(self.status), self._stream()), "paged_attention (shared)")
         self.launches += self.lib.mg_attention_shared_launches(*shape) - 1
         return out
 
@@ -1884,8 +1887,7 @@ class CudaOps:
                 raise KernelLibraryError("beam_select: no room for scores")
         if n == 0:
             return out
-        scratch = torch.empty((self.lib.mg_beam_select_scratch_bytes(groups, in_beams, beams, limit),), dtype=torch.uint8,
-                              device=self.device)
+        scratch = logits.new_empty((self.lib.mg_beam_select_scratch_bytes(groups, in_beams, beams, limit) // 4,))
         self._run(self.lib.mg_beam_select(
             _ptr(logits), _ptr(scores), _ptr(ended), _ptr(lengths), groups, in_beams, beams, vocab, limit, end, length_penalty,
             _ptr(out.tokens), _ptr(out.parents), _ptr(out.scores), _ptr(out.ranks), _ptr(out.ended), _ptr(out.lengths),

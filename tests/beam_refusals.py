@@ -92,6 +92,7 @@ def calls(ops, device):
     yield "values in the keys", attention(cache=dict(values_in_keys=True))
     yield "too few positions", attention(ctx=dict(positions=i32(2)))
     yield "too few requests", attention(ctx=dict(token_request=i32(2)))
+    yield "no groups at all", attention(ctx=dict(shared_prefix=None))
     yield "groups of two numbers", attention(groups=i32(1, 2))
     yield "no rows", attention(max_rows=0)
     yield "no keys behind", attention(max_behind=0)

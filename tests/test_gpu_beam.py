@@ -159,6 +159,23 @@ def test_attention_shared_rows_in_front_of_the_shared_end(ops, dtype):
     check_attention(case, run_attention(ops, case), dtype)
 
 
+@pytest.mark.parametrize("width", [1, 2, 8])
+def test_attention_shared_rows_of_other_widths(ops, width):
+    """Queries in rows that are wider by a few numbers: at 16-byte boundaries or not."""
+    for heads, shape in (((8, 8, 64), [(300, [3] * 80)]), ((4, 2, 48), [(70, [1, 200])])):
+        case = shared_case(shape, [], heads, 16, BF16, seed=31)
+        case.q = torch.cat([case.q, torch.full((case.q.shape[0], width), math.nan, dtype=BF16, device="cuda")], 1)
+        check_attention(case, run_attention(ops, case), BF16)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_shared_groups_that_are_none(ops, dtype):
+    """No rows, rows in front of the batch or behind it, tokens below zero or beyond any block table: the rows read all their keys."""
+    case = shared_case([], [400, 30, 90, 260], (8, 2, 64), 16, dtype, seed=32, bounds=(4, 300, 400))
+    case.ctx.shared_prefix.groups = i32([[-1, 2, 16], [0, 0, 16], [4, 3, 16], [0, 1, -5], [1, 1, 10 ** 9], [2, 2, 2 ** 31 - 1]])
+    check_attention(case, run_attention(ops, case), dtype)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_attention_shared_scores_of_large_range(ops, dtype):
     case = shared_case([(700, [30, 40, 1])], [], (4, 4, 64), 16, dtype, seed=6, spread=40.0)
