@@ -41,6 +41,7 @@ struct SharedArgs {
     int n_groups, n, n_head, n_kv_head, D, page_tokens, max_pages, num_pages, n_requests;
     int row_tiles;                     // CTAs that share the (row, head) pairs of a group
     int shared_slots, own_slots;       // ranges of the shared keys, and of a row's own
+    int page_shift;                    // page_tokens as a power of two, -1: it is none
     int shared_least;                  // keys of a range of shared keys, at least, and what they are a multiple of
     int direct;                        // every row has one range alone: the results, not parts to be joined, are left
     int first_item;                    // item of the grid's first CTA: above 0 where another kernel takes the shared ranges
@@ -147,7 +148,7 @@ __device__ __forceinline__ bool item_of(const SharedArgs& a, int item, Item& it)
 // Row of the pool, seen as [page * kv head * token][D], of the key at a position; -1: it has no page (and is not there).
 __device__ __forceinline__ int cache_row(const SharedArgs& a, const Item& it, int position, int kv_head) {
     if (position >= it.key1) return -1;
-    const int pi = position / a.page_tokens;
+    const int pi = a.page_shift >= 0 ? position >> a.page_shift : position / a.page_tokens;
     int page = pi < a.max_pages ? it.table[pi] : -1;
     if (page >= 0 && !MG_GUARDED(attention_shared, MG_GUARD_PAGE, page, a.num_pages)) page = -1;
     if (page < 0 || page >= a.num_pages) return -1;
@@ -404,6 +405,8 @@ __global__ void __launch_bounds__(MMA_THREADS) attention_shared_mma_kernel(Share
     static_assert((size_t)MMA_WARPS * NT * 8 * PSTRIDE * 4 <= Z::SMEM, "the warps' results meet where the tiles were");
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ uint32_t valid[MMA_WARPS][STAGES];
+    __shared__ int pair_token[NT * 8], pair_head[NT * 8];
+    __shared__ float weight[MMA_WARPS][NT * 8], pair_top[NT * 8], pair_sum[NT * 8];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int kv_head = blockIdx.y, share = a.n_head / a.n_kv_head, D = a.D, pieces = D / 8;
     const bf16* const k_pages = (const bf16*)a.k_pages;
@@ -582,20 +585,33 @@ __global__ void __launch_bounds__(MMA_THREADS) attention_shared_mma_kernel(Share
                 }
             }
         __syncthreads();
-        for (int e = tid; e < nts * 8 * DP; e += MMA_THREADS) {
-            const int j = e / DP, d = e % DP, token = pair_row(a, it, q0 + j, share);
-            if (token < 0 || d >= D) continue;
-            float top = -INFINITY, v = 0.f, l = 0.f;
+        // a pair's row and head, and what each warp's numbers count for
+        if (tid < NT * 8) {
+            pair_token[tid] = tid < nts * 8 ? pair_row(a, it, q0 + tid, share) : -1;
+            pair_head[tid] = kv_head * share + (q0 + tid) % share;
+            float top = -INFINITY, l = 0.f;
 #pragma unroll
-            for (int w = 0; w < MMA_WARPS; ++w) top = fmaxf(top, part[(w * NT * 8 + j) * PSTRIDE + DP]);
+            for (int w = 0; w < MMA_WARPS; ++w) top = fmaxf(top, part[(w * NT * 8 + tid) * PSTRIDE + DP]);
 #pragma unroll
             for (int w = 0; w < MMA_WARPS; ++w) {                       // warps in order
-                const float* const src = part + (w * NT * 8 + j) * PSTRIDE;
-                const float f = src[DP] == -INFINITY ? 0.f : exp2f(src[DP] - top);
-                v = fmaf(f, src[d], v);
-                l = fmaf(f, src[DP + 1], l);
+                const float ref_w = part[(w * NT * 8 + tid) * PSTRIDE + DP];
+                const float f = ref_w == -INFINITY ? 0.f : exp2f(ref_w - top);
+                weight[w][tid] = f;
+                l = fmaf(f, part[(w * NT * 8 + tid) * PSTRIDE + DP + 1], l);
             }
-            leave<bf16>(a, it, token, kv_head * share + (q0 + j) % share, d, v, top, l);
+            pair_top[tid] = top;
+            pair_sum[tid] = l;
+        }
+        __syncthreads();
+        for (int j = warp; j < nts * 8; j += MMA_WARPS) {
+            const int token = pair_token[j];
+            if (token < 0) continue;
+            for (int d = lane; d < D; d += 32) {
+                float v = 0.f;
+#pragma unroll
+                for (int w = 0; w < MMA_WARPS; ++w) v = fmaf(weight[w][j], part[(w * NT * 8 + j) * PSTRIDE + d], v);
+                leave<bf16>(a, it, token, pair_head[j], d, v, pair_top[j], pair_sum[j]);
+            }
         }
         __syncthreads();                                                // (the tiles are loaded again for the next pairs)
     }
@@ -632,7 +648,7 @@ struct TcSizes {
 };
 
 struct __align__(8) TcSync {
-    uint64_t k_full[4], v_full[4], k_free[4], v_free[4], s_full[TC_TILES][2], p_ready[TC_TILES][2], pv_done[TC_TILES], q_ready[TC_TILES], round_done[TC_TILES];
+    uint64_t kv_full[4], kv_free[4], s_full[TC_TILES][2], p_ready[TC_TILES][2], pv_done[TC_TILES], q_ready[TC_TILES], round_done[TC_TILES];
     float meet[TC_TILES][2][TC_PAIRS];      // what the two threads of a pair tell each other
     uint32_t tmem, failed;
 };
@@ -693,10 +709,8 @@ attention_shared_tc_kernel(SharedArgs a, const __grid_constant__ CUtensorMap map
 
     if (tid == 0) {
         for (int s = 0; s < STAGES; ++s) {
-            mbar_init(smem_u32(&sync.k_full[s]), 1);
-            mbar_init(smem_u32(&sync.v_full[s]), 1);
-            mbar_init(smem_u32(&sync.k_free[s]), TC_TILES);
-            mbar_init(smem_u32(&sync.v_free[s]), TC_TILES);
+            mbar_init(smem_u32(&sync.kv_full[s]), 1);
+            mbar_init(smem_u32(&sync.kv_free[s]), TC_TILES);
         }
         for (int i = 0; i < TC_TILES; ++i) {
             mbar_init(smem_u32(&sync.pv_done[i]), 1);
@@ -741,9 +755,7 @@ attention_shared_tc_kernel(SharedArgs a, const __grid_constant__ CUtensorMap map
             return w;
         };
         int n = 0, code = 0;                                            // blocks so far
-        bool holes = false;                                             // whether a page of the range is missing
-        for (int c = it.key0 / a.page_tokens + lane; c <= (it.key1 - 1) / a.page_tokens; c += 32) holes = holes || page_at(c) < 0;
-        holes = __any_sync(0xffffffffu, holes);
+        bool holes = false, looked = false;                             // whether a page of the range is missing
         for (int q0 = first_pair, round = 0; q0 < pairs && code == 0; q0 += stride, ++round) {
             const int j0 = q0 + i * TC_PAIRS;
             if (j0 >= pairs) continue;                                  // no pairs for this tile
@@ -763,6 +775,11 @@ attention_shared_tc_kernel(SharedArgs a, const __grid_constant__ CUtensorMap map
             async_proxy_fence();
             tc_fence_before();
             mbar_arrive(smem_u32(&sync.q_ready[i]));
+            if (!looked) {                                              // (while the first keys are on their way)
+                for (int c = it.key0 / a.page_tokens + lane; c <= (it.key1 - 1) / a.page_tokens; c += 32) holes = holes || page_at(c) < 0;
+                holes = __any_sync(0xffffffffu, holes);
+                looked = true;
+            }
             float ref = -INFINITY, total = 0.f;
             for (int b = 0; b < n_blocks; ++b, ++n) {
                 const int last = it.key1 - it.key0 - b * TC_KEYS;       // keys of this block
@@ -838,7 +855,7 @@ attention_shared_tc_kernel(SharedArgs a, const __grid_constant__ CUtensorMap map
                 // the same zeros: neither waits for the other)
                 if (last < TC_KEYS && h == 0) {
                     const int stage = n % STAGES;
-                    if (!warp_wait(smem_u32(&sync.v_full[stage]), (n / STAGES) & 1)) code = 65;
+                    if (!warp_wait(smem_u32(&sync.kv_full[stage]), (n / STAGES) & 1)) code = 65;
                     if (mine >= last && mine < TC_KEYS)
 #pragma unroll
                         for (int atom = 0; atom < ATOMS; ++atom)
@@ -907,83 +924,74 @@ attention_shared_tc_kernel(SharedArgs a, const __grid_constant__ CUtensorMap map
                     if (a.page_tokens < TC_KEYS) column += boxes;
                     else if ((offset += TC_KEYS) >= a.page_tokens) { offset = 0; ++column; }
                     page = look();
+                    if (n >= STAGES && !warp_wait(smem_u32(&sync.kv_free[stage]), (n / STAGES - 1) & 1)) { code = 60; break; }
+                    const uint32_t full = smem_u32(&sync.kv_full[stage]);
+                    if (lane == 0) mbar_expect_tx(full, 2 * Z::TILE);
+                    __syncwarp();
+                    if (lane < boxes)
 #pragma unroll
-                    for (int which = 0; which < 2; ++which) {
-                        uint64_t* const full = which ? &sync.v_full[stage] : &sync.k_full[stage];
-                        uint64_t* const free = which ? &sync.v_free[stage] : &sync.k_free[stage];
-                        if (n >= STAGES && !warp_wait(smem_u32(free), (n / STAGES - 1) & 1)) { code = 60; break; }
-                        if (lane == 0) mbar_expect_tx(smem_u32(full), Z::TILE);
-                        __syncwarp();
-                        if (lane < boxes)
-#pragma unroll
-                            for (int atom = 0; atom < ATOMS; ++atom)
-                                tma_load_2d(smem_u32((which ? v_tiles : k_tiles) + stage * Z::TILE + atom * Z::ATOM + lane * box_rows * 128),
-                                            which ? &map_v : &map_k, smem_u32(full), atom * 64, y);
-                        __syncwarp();
-                    }
+                        for (int atom = 0; atom < ATOMS; ++atom) {
+                            const uint32_t off = stage * Z::TILE + atom * Z::ATOM + lane * box_rows * 128;
+                            tma_load_2d(smem_u32(k_tiles) + off, &map_k, full, atom * 64, y);
+                            tma_load_2d(smem_u32(v_tiles) + off, &map_v, full, atom * 64, y);
+                        }
+                    __syncwarp();
                 }
             }
-        } else {
-            // a warp a tile: each waits for its own softmax and products, so that the other's fill the time
+        } else if (elect_one()) {
+            // One thread a tile issues its products and waits for its own softmax and products alone, so that the other tile's
+            // fill the time.
             const int i = warp - TC_ISSUE;
             int n = 0;
             for (int q0 = first_pair, round = 0; q0 < pairs && code == 0; q0 += stride, ++round) {
-                const bool active = q0 + i * TC_PAIRS < pairs;
-                auto scores = [&](int m) {                              // S of block m = Q K^T
+                auto scores = [&](int m) {                              // S of block m = Q K^T, once its keys and values are there
                     const int stage = m % STAGES;
-                    if (!warp_wait(smem_u32(&sync.k_full[stage]), (m / STAGES) & 1)) return false;
+                    if (!mbar_wait(smem_u32(&sync.kv_full[stage]), (m / STAGES) & 1)) return false;
                     tc_fence_after();
-                    if (elect_one()) {
-                        constexpr uint32_t idesc = instr_desc_bf16(TC_PAIRS, TC_KEYS, false);
-                        const uint64_t dq = smem_desc_sw128(smem_u32(q_tiles + i * Z::Q_TILE)), dk = smem_desc_sw128(smem_u32(k_tiles + stage * Z::TILE));
+                    constexpr uint32_t idesc = instr_desc_bf16(TC_PAIRS, TC_KEYS, false);
+                    const uint64_t dq = smem_desc_sw128(smem_u32(q_tiles + i * Z::Q_TILE)), dk = smem_desc_sw128(smem_u32(k_tiles + stage * Z::TILE));
 #pragma unroll
-                        for (int k = 0; k < D / 16; ++k)
-                            umma_bf16(tmem + (i * 2 + (m & 1)) * TC_KEYS, dq + (uint64_t)((k / 4 * Z::Q_ATOM + k % 4 * 32) >> 4),
-                                      dk + (uint64_t)((k / 4 * Z::ATOM + k % 4 * 32) >> 4), idesc, k ? 1u : 0u);
-                        umma_commit(smem_u32(&sync.s_full[i][m & 1]));
-                        umma_commit(smem_u32(&sync.k_free[stage]));
-                    }
-                    __syncwarp();
+                    for (int k = 0; k < D / 16; ++k)
+                        umma_bf16(tmem + (i * 2 + (m & 1)) * TC_KEYS, dq + (uint64_t)((k / 4 * Z::Q_ATOM + k % 4 * 32) >> 4),
+                                  dk + (uint64_t)((k / 4 * Z::ATOM + k % 4 * 32) >> 4), idesc, k ? 1u : 0u);
+                    umma_commit(smem_u32(&sync.s_full[i][m & 1]));
                     return true;
                 };
-                if (!active) {                                          // no pairs for this tile: it gives the blocks back unread
+                if (q0 + i * TC_PAIRS >= pairs) {                       // no pairs for this tile: it gives the blocks back unread
                     for (int b = 0; b < n_blocks && code == 0; ++b, ++n) {
-                        const int stage = n % STAGES;
-                        if (!warp_wait(smem_u32(&sync.k_full[stage]), (n / STAGES) & 1) || !warp_wait(smem_u32(&sync.v_full[stage]), (n / STAGES) & 1)) {
-                            code = 61;
-                        } else if (lane == 0) {
-                            mbar_arrive(smem_u32(&sync.k_free[stage]));
-                            mbar_arrive(smem_u32(&sync.v_free[stage]));
-                        }
+                        if (!mbar_wait(smem_u32(&sync.kv_full[n % STAGES]), (n / STAGES) & 1)) code = 61;
+                        else mbar_arrive(smem_u32(&sync.kv_free[n % STAGES]));
                     }
                     continue;
                 }
-                if (!warp_wait(smem_u32(&sync.q_ready[i]), round & 1)) { code = 67; break; }
+                if (!mbar_wait(smem_u32(&sync.q_ready[i]), round & 1)) { code = 67; break; }
                 if (!scores(n) || (n_blocks > 1 && !scores(n + 1))) code = 61;
                 for (int b = 0; b < n_blocks && code == 0; ++b, ++n) {
                     const int stage = n % STAGES;
-                    if (!warp_wait(smem_u32(&sync.p_ready[i][n & 1]), (n >> 1) & 1)) { code = 62; break; }
-                    if (!warp_wait(smem_u32(&sync.v_full[stage]), (n / STAGES) & 1)) { code = 63; break; }
+                    if (!mbar_wait(smem_u32(&sync.p_ready[i][n & 1]), (n >> 1) & 1)) { code = 62; break; }
                     tc_fence_after();
-                    if (elect_one()) {
-                        constexpr uint32_t idesc = instr_desc_bf16(TC_PAIRS, D, true);
-                        // (values: atoms of 64 features, the second an atom's bytes behind the first)
-                        const uint64_t dv = smem_desc_sw128(smem_u32(v_tiles + stage * Z::TILE)) + ((uint64_t)((Z::ATOM >> 4) - 1) << 16);
+                    constexpr uint32_t idesc = instr_desc_bf16(TC_PAIRS, D, true);
+                    // (values: atoms of 64 features, the second an atom's bytes behind the first)
+                    const uint64_t dv = smem_desc_sw128(smem_u32(v_tiles + stage * Z::TILE)) + ((uint64_t)((Z::ATOM >> 4) - 1) << 16);
 #pragma unroll
-                        for (int k = 0; k < TC_KEYS / 16; ++k)
-                            umma_bf16_ts(tmem + TC_O_COL + i * D, tmem + (i * 2 + (n & 1)) * TC_KEYS + (k / 2) * (TC_KEYS / 2) + (k % 2) * 8, dv + (uint64_t)(k * (16 * 128) >> 4), idesc,
-                                         (b | k) ? 1u : 0u);
-                        umma_commit(smem_u32(&sync.pv_done[i]));
-                        umma_commit(smem_u32(&sync.v_free[stage]));
-                        if (b == n_blocks - 1) umma_commit(smem_u32(&sync.round_done[i]));
-                    }
-                    __syncwarp();
+                    for (int k = 0; k < TC_KEYS / 16; ++k)
+                        umma_bf16_ts(tmem + TC_O_COL + i * D, tmem + (i * 2 + (n & 1)) * TC_KEYS + (k / 2) * (TC_KEYS / 2) + (k % 2) * 8,
+                                     dv + (uint64_t)(k * (16 * 128) >> 4), idesc, (b | k) ? 1u : 0u);
+                    umma_commit(smem_u32(&sync.pv_done[i]));
+                    umma_commit(smem_u32(&sync.kv_free[stage]));
+                    if (b == n_blocks - 1) umma_commit(smem_u32(&sync.round_done[i]));
                     // the scores of the block after the next, in the place of the P that has just gone into the average (only the wait
                     // orders the two)
-                    if (b + 2 < n_blocks && (!warp_wait(smem_u32(&sync.pv_done[i]), n & 1) || !scores(n + 2))) code = 61;
+                    if (b + 2 < n_blocks && (!mbar_wait(smem_u32(&sync.pv_done[i]), n & 1) || !scores(n + 2))) code = 61;
                 }
             }
+            if (code) {
+                atomicExch(status, code);
+                *(volatile uint32_t*)&sync.failed = 1;
+            }
+            code = 0;
         }
+        __syncwarp();
         if (code && lane == 0) {
             atomicExch(status, code);
             *(volatile uint32_t*)&sync.failed = 1;
@@ -1238,6 +1246,7 @@ MG_API int mg_attention_shared(const void* q, long long q_stride, const void* k_
     MG_REQUIRE(c.direct || scratch != nullptr, "attention (shared): no scratch");
     if (c.direct) a.n_groups = n_groups = 0;
     a.direct = c.direct; a.element = is_bf16 ? 2 : 4;
+    a.page_shift = (page_tokens & (page_tokens - 1)) == 0 ? __builtin_ctz(page_tokens) : -1;
     a.first_item = 0; a.shared_least = c.shared_least;
     a.row_tiles = c.row_tiles; a.shared_slots = c.shared_slots; a.own_slots = c.own_slots;
     a.scale_log2e = scale * 1.4426950408889634f;
