@@ -179,7 +179,7 @@ __device__ __forceinline__ void leave(const SharedArgs& a, const Item& it, int r
 // ---- any head size, either type: 8 or 16 (row, head) pairs and 64 keys at a time, in 32-bit arithmetic -------------------
 // The 32-bit mode's kernel, and that of bfloat16 heads whose size is no multiple of 8.  Keys and values of a block come to
 // shared memory together, several loads a thread on their way (read one by one where they are used: 27 us for 10 rows of
-// some 530 keys and 12 heads of 64, where this takes SIMT_US).  Scores: a thread a key and half of the pairs; average: a thread a
+// some 530 keys and 12 heads of 64, where this takes 14).  Scores: a thread a key and half of the pairs; average: a thread a
 // feature and all pairs.
 constexpr int SIMT_THREADS = 128;
 

@@ -132,3 +132,24 @@ def test_beams_of_heads_and_rows_that_the_tiles_take():
         for a, b in zip(with_tiles, without):
             assert a["logprob"] == pytest.approx(b["logprob"], abs=12 * 2 * 8e-3)
         assert math.isfinite(with_tiles[-1]["logprob"])
+
+
+def test_beam_search_by_the_command_line(tmp_path):
+    import json
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    from harness import make_model_dir, tokens_for
+    import plain_gpt
+
+    folder, cfg, tensors = make_model_dir(tmp_path, "A", 31, "float32")
+    prompt = tokens_for(cfg, 9, 4)
+    cmd = [sys.executable, str(Path(__file__).resolve().parent.parent / "bin" / "generate"), "--model", str(folder), "--prompt-ids",
+           ",".join(map(str, prompt)), "--beams", "3", "--max-new-tokens", "6", "--dtype", "float32", "--kv-block-size", "8",
+           "--num-kv-blocks", "64"]
+    proc = subprocess.run(cmd, capture_output=True, text=True, timeout=600)
+    assert proc.returncode == 0, proc.stderr[-2000:]
+    out = json.loads([line for line in proc.stdout.splitlines() if line.startswith("{")][0])
+    last = lambda tokens: plain_gpt.forward_logits(tokens, tensors, cfg.n_layer, cfg.n_head, cfg.layer_norm_epsilon)[-1]  # noqa: E731
+    check(out["beams"], plain_beam.search(last, prompt, 3, 6))
