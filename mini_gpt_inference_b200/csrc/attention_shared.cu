@@ -1127,7 +1127,7 @@ int launch_simt(const SharedArgs& a, int pairs, cudaStream_t s) {
                    : launch_ranges(attention_shared_simt_kernel<T, 16, VEC>, SIMT_THREADS, smem, a, s);
 }
 
-constexpr int DIRECT_KEYS = 256, TC_LEAST_PAIRS = 64, TC_CTA_KEYS = 1000;
+constexpr int DIRECT_KEYS = 256, DIRECT_ROWS = 256, TC_LEAST_PAIRS = 32, TC_CTA_KEYS = 1000;
 
 template <int DP>
 int launch_mma(const SharedArgs& a, int pair_tiles, cudaStream_t s) {
@@ -1160,11 +1160,16 @@ struct Cut {
 Cut cut(int n_groups, int max_rows, int max_tokens, int max_behind, int n, int n_head, int n_kv_head, int head_dim, int page_tokens,
         int kind) {
     Cut c;
-    // So few keys that reading them once a row costs less than a second kernel.
-    c.direct = (n_groups == 0 ? max_behind : max_tokens + max_behind) <= DIRECT_KEYS;
+    // So few keys that reading them once a row costs less than a second kernel.  (8 heads of 64, two kernels / one, us: 4 rows of 94
+    // keys 6.5 / 4.8, of 256 7.0 / 6.4, of 512 7.8 / 9.1; 64 rows of 256 11.3 / 8.1, of 1,024 14.3 / 19.0; 256 rows of 128
+    // 25.7 / 19.2, of 256 26.3 / 26.0, of 512 39.8 / 38.3; 512 rows of 128 36.9 / 34.5, of 190 38.2 / 41.3.)
+    const long long keys = n_groups == 0 ? max_behind : (long long)max_tokens + max_behind;
+    c.direct = keys <= DIRECT_KEYS / 2 || (keys <= DIRECT_KEYS && (n_groups == 0 || n <= DIRECT_ROWS));
     if (c.direct) n_groups = 0;
     const int share = n_head / n_kv_head, pairs = n_groups > 0 ? (max_rows < n ? max_rows : n) * share : share;
     c.mma = kind == BF16_ALIGNED && head_dim % 8 == 0;
+    // tcgen05 from 32 pairs on.  (mma.sync / tcgen05, us, 2,000 shared tokens: 8 heads of 64, 16 pairs 18.1 / 19.3, 32 22.2 / 16.0, 128
+    // 32.0 / 22.9; 32/8 heads of 128, 16 pairs 23.5 / 19.1 and with 300 tokens 12.3 / 14.6, 32 32.1 / 21.5, 512 76 / 36.5.)
     c.tc = n_groups > 0 && kind == BF16_ALIGNED && (head_dim == 64 || head_dim == 128) && pairs >= TC_LEAST_PAIRS && page_tokens % 8 == 0 &&
            (page_tokens < TC_KEYS ? TC_KEYS % page_tokens == 0 : page_tokens % TC_KEYS == 0) && max_tokens >= TC_KEYS;
     const int most_tiles = head_dim <= 64 ? 4 : head_dim <= 128 ? 2 : 1;      // what the registers hold
