@@ -7,7 +7,7 @@
 // logits, equal ones by the lower id, so a row's B largest logits are all that a row can contribute, whatever L_b is:
 //
 //   rows kernel    one pass over the logits: every lane of a CTA keeps the maximum and sum of its own (for L_b).  The B best
-//                  logits of the CTA's piece lie in the B lanes with the largest maxima; those lanes' logits are looked at again.
+//                  logits of the CTA's piece lie in the lanes with the B largest maxima; those lanes' logits are looked at again.
 //                  (logit, id) pairs are 64-bit keys, the logit's bits in an order that unsigned numbers have, then the id
 //                  from above: all keys differ, so ties need no care.  Lists are sorted over a warp's lanes and joined by
 //                  bitonic merges.  (Every warp keeping the B best of its piece as it reads: 768 instructions for 512 logits
@@ -62,20 +62,30 @@ __device__ __forceinline__ u64 merge_lists(u64 a, u64 b, int lane) {
     return c;
 }
 
-// The lanes' keys sorted downwards.
-__device__ __forceinline__ u64 sort_lanes(u64 v, int lane) {
+// The 32 largest of two lists of numbers, and the lanes' numbers, sorted downwards over the lanes.
+__device__ __forceinline__ uint32_t merge_lists(uint32_t a, uint32_t b, int lane) {
+    uint32_t c = max(a, __shfl_xor_sync(0xffffffffu, b, 31));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, c, o);
+        c = (lane & o) ? min(c, other) : max(c, other);
+    }
+    return c;
+}
+__device__ __forceinline__ uint32_t sort_lanes(uint32_t v, int lane) {
 #pragma unroll
     for (int k = 2; k <= 32; k <<= 1)
 #pragma unroll
         for (int o = k >> 1; o > 0; o >>= 1) {
-            const u64 other = __shfl_xor_sync(0xffffffffu, v, o);
-            v = ((lane & k) == 0) == ((lane & o) == 0) ? max64(v, other) : min64(v, other);
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, v, o);
+            v = ((lane & k) == 0) == ((lane & o) == 0) ? max(v, other) : min(v, other);
         }
     return v;
 }
 
 // The 32 largest keys of the CTA's warps, sorted downwards over the lanes of warp 0, from lists that are so in every warp.
-__device__ __forceinline__ u64 merge_warps(u64 list, u64 (&meet)[ROW_WARPS][32], int warp, int lane) {
+template <typename T>
+__device__ __forceinline__ T merge_warps(T list, T (&meet)[ROW_WARPS][32], int warp, int lane) {
     meet[warp][lane] = list;
 #pragma unroll
     for (int half = ROW_WARPS / 2; half > 0; half >>= 1) {
@@ -91,7 +101,8 @@ __device__ __forceinline__ u64 merge_warps(u64 list, u64 (&meet)[ROW_WARPS][32],
 __global__ void __launch_bounds__(ROW_THREADS)
 beam_rows_kernel(const float* __restrict__ logits, const int* __restrict__ ended, u64* __restrict__ lists, float* __restrict__ sums,
                  int vocab, int limit, int beams, int chunk) {
-    __shared__ u64 meet[ROW_WARPS][32], lanes_in_order[32];
+    __shared__ u64 meet[ROW_WARPS][32];
+    __shared__ uint32_t meet_order[ROW_WARPS][32], owners[ROW_WARPS][2], bound_s;
     __shared__ float meet_max[ROW_WARPS], meet_sum[ROW_WARPS];
     const int row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_wait();
@@ -114,7 +125,6 @@ beam_rows_kernel(const float* __restrict__ logits, const int* __restrict__ ended
         }
     };
     float top = -INFINITY, sum = 0.f, next_x[4][4];
-    int top_batch = begin;
     if (begin < end)
 #pragma unroll
         for (int q = 0; q < 4; ++q) quad(begin + q * 128 + lane * 4, next_x[q]);
@@ -131,7 +141,6 @@ beam_rows_kernel(const float* __restrict__ logits, const int* __restrict__ ended
         if (high > top) {                                   // the sum is relative to the largest so far
             sum *= exp2f((top - high) * log2e);
             top = high;
-            top_batch = b0;
         }
         const float shift = top == -INFINITY ? 0.f : top * log2e;
         float part[4] = {0.f, 0.f, 0.f, 0.f};
@@ -142,60 +151,57 @@ beam_rows_kernel(const float* __restrict__ logits, const int* __restrict__ ended
     const float warp_top = warp_max(top);
     sum = warp_sum(warp_top == -INFINITY ? 0.f : sum * exp2f((top - warp_top) * log2e));
     if (lane == 0) { meet_max[warp] = warp_top; meet_sum[warp] = sum; }
-    // The key of the lane's largest logit: the first of its batch that is as large.
-    u64 key = 0;
-#pragma unroll
-    for (int q = 3; q >= 0; --q) {
-        float x[4];
-        const int at = top_batch + q * 128 + lane * 4;
-        quad(at, x);
-#pragma unroll
-        for (int i = 3; i >= 0; --i)
-            if (at + i >= lead && at + i < end && fmaxf(x[i], -INFINITY) == top) key = key_of(top, at + i - lead);
+    // The CTA's 256 lanes have `beams` logits not below the beams-th largest of their maxima: what is as good lies in the lanes
+    // whose maximum is, and their logits are looked at once more, a lane's by a warp.  (Lanes without logits count as minus
+    // infinity here and add nothing there; where fewer than `beams` lanes have some, that is the bound.)  Equal logits go by their
+    // ids, which rise with the warps: once `beams` lanes reach the bound, later warps' lanes have to pass it.  (64 x 16
+    // rows of 50,257 equal logits, or of all but three minus infinity, together with the launches: 104 us, 212 without that.)
+    const uint32_t maxima = merge_warps(sort_lanes(order_of(top), lane), meet_order, warp, lane);
+    if (warp == 0) {
+        const uint32_t bound = __shfl_sync(0xffffffffu, maxima, beams - 1);
+        if (lane == 0) bound_s = bound;
     }
-    // The CTA's 256 lanes have `beams` logits not below the beams-th largest of those: what is as good lies in the lanes of the
-    // first `beams` of them (all keys differ), whose logits are looked at once more, a lane's by a warp.
-    const u64 best_lane = merge_warps(sort_lanes(key, lane), meet, warp, lane);
-    if (warp == 0) lanes_in_order[lane] = best_lane;
     __syncthreads();
-    const u64 bound = lanes_in_order[beams - 1];
+    const float bound = number_of(bound_s);
+    const uint32_t good = __ballot_sync(0xffffffffu, begin < end && top >= bound), better = __ballot_sync(0xffffffffu, top > bound);
+    if (lane == 0) { owners[warp][0] = good; owners[warp][1] = better; }
+    __syncthreads();
     u64 list = 0, least = 0;                                // lane i: the warp's i-th best; its beams-th best
-    for (int k = warp; k < beams; k += ROW_WARPS) {
-        const u64 owner = lanes_in_order[k];
-        if (owner == 0) break;
-        const int cta = blockIdx.x * ROW_WARPS * chunk, at = (int)~(uint32_t)owner + lead - cta;      // where the lane's best lies
-        const int first = cta + at / chunk * chunk, column = first + at % chunk % 128 / 4 * 4, last = min(limit + lead, first + chunk);
-        for (int q = lane; q < chunk / 128 + lane; q += 32) {      // (whole warps)
-            const int j = column + q * 128;
-            float x[4];
-            const bool there = q < chunk / 128;
+    int turn = 0, reach = 0;                                // lanes taken; lanes of the warps so far that reach the bound
+    for (int w = 0; w < ROW_WARPS; ++w) {
+        const int first = (blockIdx.x * ROW_WARPS + w) * chunk, last = min(limit + lead, first + chunk);
+        uint32_t left = owners[w][reach >= beams];
+        reach += __popc(owners[w][0]);
+        for (; left; left &= left - 1, ++turn) {
+            if (turn % ROW_WARPS != warp) continue;
+            const int column = first + (__ffs(left) - 1) * 4;
+            for (int j = column + lane * 128; __any_sync(0xffffffffu, j < last); j += 32 * 128) {
+                float x[4];
+                if (j >= lead && j + 4 <= last) {
+                    const float4 v = *reinterpret_cast<const float4*>(base + (j - lead));
+                    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+                } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = -INFINITY;
-            if (there && j >= lead && j + 4 <= last) {
-                const float4 v = *reinterpret_cast<const float4*>(base + (j - lead));
-                x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-            } else if (there) {
+                    for (int i = 0; i < 4; ++i) x[i] = (j + i >= lead && j + i < last) ? base[j + i - lead] : -INFINITY;
+                }
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (j + i >= lead && j + i < last) x[i] = base[j + i - lead];
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const u64 mine = there && j + i >= lead && j + i < last ? key_of(fmaxf(x[i], -INFINITY), j + i - lead) : 0;
-                uint32_t todo = __ballot_sync(0xffffffffu, mine != 0 && mine >= bound && mine > least);
-                while (todo) {
-                    const u64 next = __shfl_sync(0xffffffffu, mine, __ffs(todo) - 1);
-                    todo &= todo - 1;
-                    if (next <= least) continue;            // (the list has grown since the ballot)
-                    const int place = __popc(__ballot_sync(0xffffffffu, list > next));
-                    const u64 up = __shfl_up_sync(0xffffffffu, list, 1);
-                    list = lane < place ? list : lane == place ? next : up;
-                    least = __shfl_sync(0xffffffffu, list, beams - 1);
+                for (int i = 0; i < 4; ++i) {
+                    x[i] = fmaxf(x[i], -INFINITY);
+                    const u64 mine = x[i] >= bound && j + i >= lead && j + i < last ? key_of(x[i], j + i - lead) : 0;
+                    uint32_t todo = __ballot_sync(0xffffffffu, mine > least);
+                    while (todo) {
+                        const u64 next = __shfl_sync(0xffffffffu, mine, __ffs(todo) - 1);
+                        todo &= todo - 1;
+                        if (next <= least) continue;        // (the list has grown since the ballot)
+                        const int place = __popc(__ballot_sync(0xffffffffu, list > next));
+                        const u64 up = __shfl_up_sync(0xffffffffu, list, 1);
+                        list = lane < place ? list : lane == place ? next : up;
+                        least = __shfl_sync(0xffffffffu, list, beams - 1);
+                    }
                 }
             }
         }
     }
-    __syncthreads();                                        // (the lanes' lists have been read)
     list = merge_warps(list, meet, warp, lane);
     if (warp == 0) {
         const size_t at = (size_t)row * gridDim.x + blockIdx.x;

@@ -331,6 +331,29 @@ def test_beam_select_ties_and_odd_numbers(ops, what):
     check_choice(got, plain_beam.beam_select(logits, scores, beams), groups, beams)
 
 
+@pytest.mark.parametrize("beams", [5, 32])
+@pytest.mark.parametrize("what", ["equal", "few allowed", "few values", "last one", "two values"])
+def test_beam_select_ties_over_a_long_row(ops, what, beams):
+    """Ties over several pieces of a row: the lowest ids go on, wherever they lie."""
+    gen = torch.Generator().manual_seed(beams)
+    groups, in_beams, vocab = 2, 3, 50257
+    logits = torch.randn(groups * in_beams, vocab, generator=gen)
+    scores = -3 * torch.rand(groups, in_beams, generator=gen)
+    if what == "equal":
+        logits[:] = -1.5
+    elif what == "few allowed":
+        logits[:, torch.randperm(vocab, generator=gen)[3:]] = -math.inf
+    elif what == "few values":
+        logits = (logits * 2).round()
+    elif what == "last one":
+        logits[:] = 0.0
+        logits[:, -1] = 1.0
+    elif what == "two values":
+        logits = (torch.rand(groups * in_beams, vocab, generator=gen) < 0.01).float()
+    got = ops.beam_select(logits.cuda(), scores.cuda(), beams)
+    check_choice(got, plain_beam.beam_select(logits, scores, beams), groups, beams)
+
+
 def test_beam_select_all_ended_and_unaligned_rows(ops):
     logits = torch.randn(4 * 777 + 1, generator=torch.Generator().manual_seed(1))
     view = logits.cuda()[1:].view(4, 777)                                   # starts four bytes behind a boundary
