@@ -388,17 +388,21 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 
 constexpr int MMA_THREADS = 128, MMA_WARPS = MMA_THREADS / 32, UNIT = 16;       // keys a warp takes at a time
 
-// Sizes by padded head: DP features (32, 64, 128 or 256), of which D are there and the others zero.
-template <int DP>
+// Sizes by padded head: DP features (32, 64, 128 or 256), of which D are there and the others zero; and the CTAs that an SM is to
+// hold.  A CTA of few keys is mostly its chain of trips to memory (which range, its group, the pages, the keys), so many small
+// rings an SM hide more than deep ones: heads of 64 at six CTAs of two stages instead of four of three 13.7 -> 11.6 us for 64 rows
+// of 1,021 tokens.  Heads of 128 take one stage at six CTAs (MANY) or two at three: see cut().
+template <int DP, int NT, bool MANY>
 struct MmaSizes {
-    static constexpr int STAGES = DP == 32 ? 4 : DP == 64 ? 3 : 2;
+    static constexpr int STAGES = DP == 32 ? 4 : DP == 64 ? (NT == 1 ? 2 : 3) : MANY ? 1 : 2;
+    static constexpr int CTAS = DP == 32 ? (NT == 1 ? 8 : NT == 2 ? 5 : 4) : DP == 64 ? (NT == 1 ? 6 : NT == 2 ? 4 : 3) : MANY ? 6 : DP == 128 && NT == 1 ? 3 : 2;
     static constexpr int TILE = UNIT * DP * 2;                          // bytes of 16 keys or values
     static constexpr size_t SMEM = (size_t)MMA_WARPS * STAGES * 2 * TILE;
 };
 
-template <int DP, int NT>      // NT: tiles of 8 pairs that a CTA takes at once
-__global__ void __launch_bounds__(MMA_THREADS) attention_shared_mma_kernel(SharedArgs a) {
-    using Z = MmaSizes<DP>;
+template <int DP, int NT, bool MANY>      // NT: tiles of 8 pairs that a CTA takes at once
+__global__ void __launch_bounds__(MMA_THREADS, MmaSizes<DP, NT, MANY>::CTAS) attention_shared_mma_kernel(SharedArgs a) {
+    using Z = MmaSizes<DP, NT, MANY>;
     constexpr int STAGES = Z::STAGES, CPR = DP / 8, ROWB = 2 * DP;
     constexpr int RPL = CPR >= 8 ? 1 : 8 / CPR, SWZ = CPR >= 8 ? 8 : CPR;     // piece c of row r lies at piece c ^ ((r / RPL) % SWZ)
     constexpr int PSTRIDE = DP + 2;                                     // floats of a warp's partial: O, maximum, sum
@@ -1129,14 +1133,19 @@ int launch_simt(const SharedArgs& a, int pairs, cudaStream_t s) {
 
 constexpr int DIRECT_KEYS = 256, DIRECT_ROWS = 256, TC_LEAST_PAIRS = 32, TC_CTA_KEYS = 1000;
 
+template <int DP, int NT, bool MANY>
+int launch_mma_tiles(const SharedArgs& a, cudaStream_t s) {
+    return launch_ranges(attention_shared_mma_kernel<DP, NT, MANY>, MMA_THREADS, MmaSizes<DP, NT, MANY>::SMEM, a, s);
+}
 template <int DP>
-int launch_mma(const SharedArgs& a, int pair_tiles, cudaStream_t s) {
-    constexpr size_t smem = MmaSizes<DP>::SMEM;
-    if (pair_tiles == 1) return launch_ranges(attention_shared_mma_kernel<DP, 1>, MMA_THREADS, smem, a, s);
+int launch_mma(const SharedArgs& a, int pair_tiles, bool many, cudaStream_t s) {
+    if constexpr (DP == 128)
+        if (pair_tiles == 1 && many) return launch_mma_tiles<DP, 1, true>(a, s);
+    if (pair_tiles == 1) return launch_mma_tiles<DP, 1, false>(a, s);
     if constexpr (DP <= 128)
-        if (pair_tiles == 2) return launch_ranges(attention_shared_mma_kernel<DP, 2>, MMA_THREADS, smem, a, s);
+        if (pair_tiles == 2) return launch_mma_tiles<DP, 2, false>(a, s);
     if constexpr (DP <= 64)
-        if (pair_tiles == 4) return launch_ranges(attention_shared_mma_kernel<DP, 4>, MMA_THREADS, smem, a, s);
+        if (pair_tiles == 4) return launch_mma_tiles<DP, 4, false>(a, s);
     return mg_set_error(MG_ERR_ARG, "attention (shared): no kernel for %d tiles of pairs", pair_tiles);
 }
 
@@ -1151,6 +1160,7 @@ struct Cut {
     bool direct;         // a range a row, no groups: one launch
     bool mma, tc;        // the warp-level tensor cores; shared ranges on tcgen05
     int pair_tiles;      // mma: tiles of 8 pairs that a CTA takes at once
+    bool many;           // mma: many CTAs of few keys
     int row_tiles;       // CTAs that share the pairs of a group
     int shared_slots, own_slots;      // ranges of shared keys, and of a row's own
     int shared_least;
@@ -1194,6 +1204,11 @@ Cut cut(int n_groups, int max_rows, int max_tokens, int max_behind, int n, int n
     const long long y = (want + own_ctas - 1) / own_ctas;
     c.shared_slots = (int)(x < 1 ? 1 : x > most_shared ? most_shared : x);
     c.own_slots = c.direct ? 1 : (int)(y < 1 ? 1 : y > most_own ? most_own : y);
+    // More CTAs than three an SM, none of more than 512 keys.  (Heads of 128, a CTA a row of 8 pairs or fewer, three CTAs an SM / six:
+    // 2,048 CTAs of 128 keys 38 / 31 us, 832 of 200 20.5 / 18.1; 832 of 800 37.4 / 40.6, 328 of 865 36 / 44.6.)
+    const long long mma_ctas = own_ctas * c.own_slots + (c.tc ? 0 : shared_ctas * c.shared_slots);
+    const int range = max(ceil_div(max_behind, c.own_slots), c.tc ? 0 : ceil_div(max_tokens, c.shared_slots));
+    c.many = mma_ctas > 148 * 3 && range <= 512;
     c.pairs = pairs;
     return c;
 }
@@ -1272,10 +1287,10 @@ MG_API int mg_attention_shared(const void* q, long long q_stride, const void* k_
     }
     if (c.mma) {
         switch (padded_head(head_dim)) {
-            case 32: rc = launch_mma<32>(a, c.pair_tiles, s); break;
-            case 64: rc = launch_mma<64>(a, c.pair_tiles, s); break;
-            case 128: rc = launch_mma<128>(a, c.pair_tiles, s); break;
-            default: rc = launch_mma<256>(a, c.pair_tiles, s);
+            case 32: rc = launch_mma<32>(a, c.pair_tiles, c.many, s); break;
+            case 64: rc = launch_mma<64>(a, c.pair_tiles, c.many, s); break;
+            case 128: rc = launch_mma<128>(a, c.pair_tiles, c.many, s); break;
+            default: rc = launch_mma<256>(a, c.pair_tiles, c.many, s);
         }
     } else {
         rc = is_bf16 ? launch_simt<bf16, false>(a, c.pairs, s)

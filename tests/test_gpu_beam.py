@@ -263,6 +263,14 @@ def test_attention_shared_through_paged_attention(ops, dtype):
     check_attention(case, ops.paged_attention(case.q, H, KV, D, D ** -0.5, case.cache, case.ctx), dtype)
 
 
+@pytest.mark.parametrize("heads,rows,shared,page", [((8, 8, 96), 8, 300, 16), ((8, 8, 128), 5, 1000, 5), ((16, 8, 104), 4, 140, 64)])
+def test_attention_shared_many_short_ranges(ops, heads, rows, shared, page):
+    """So many CTAs of few keys that they take the smallest rings: ranges of no, one and some keys, features padded to 128."""
+    groups = [(shared - 7 * i, [1 + (11 * i + 5 * j) % 90 for j in range(rows)]) for i in range(8)] + [(1, [1, 1, 129])]
+    case = shared_case(groups, [1, 16, 17, 200] * 8, heads, page, BF16, seed=shared, pad=2)
+    check_attention(case, run_attention(ops, case), BF16)
+
+
 # ---- the choice of the next beams -----------------------------------------------------------------------
 def check_choice(got, want, groups, beams):
     for name in ("tokens", "parents", "ranks", "ended", "lengths"):
