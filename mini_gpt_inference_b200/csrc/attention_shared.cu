@@ -1251,7 +1251,8 @@ MG_API int mg_attention_shared(const void* q, long long q_stride, const void* k_
     MG_REQUIRE(n > 0 && n_head > 0 && n_kv_head > 0 && head_dim > 0 && page_tokens > 0 && max_pages > 0 && num_pages > 0 && n_requests > 0,
                "attention (shared): bad sizes");
     MG_REQUIRE(n_head % n_kv_head == 0, "attention: n_head %d is not a multiple of n_kv_head %d", n_head, n_kv_head);
-    MG_REQUIRE(n_groups >= 0 && (n_groups == 0 || (groups && max_rows > 0 && max_tokens >= 0)) && max_behind > 0,
+    MG_REQUIRE(n_groups >= 0 && (n_groups == 0 || (groups && max_rows > 0 && max_tokens >= 0)) && max_behind > 0 &&
+                   max_tokens <= (1 << 30) && max_behind <= (1 << 30),
                "attention (shared): bad groups or bounds");
     MG_REQUIRE(q_stride >= (long long)n_head * head_dim, "attention (shared): rows too narrow");
     MG_REQUIRE((long long)num_pages * n_kv_head * page_tokens < (1ll << 31), "attention (shared): the pool has too many rows");

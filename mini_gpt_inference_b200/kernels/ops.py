@@ -992,7 +992,8 @@ class CudaOps:
         out = qkv.new_empty((n, n_head * head_dim))
         if n == 0:
             return out
-        sizes = (groups.shape[0], int(shared.max_rows), int(shared.max_tokens), int(shared.max_behind))
+        most = min(max(1, table.shape[1] * cache.page_tokens), 1 << 30)  # (no request has more keys than its table leads to)
+        sizes = (groups.shape[0], min(int(shared.max_rows), n), min(int(shared.max_tokens), most), min(int(shared.max_behind), most))
         shape = (*sizes, n, n_head, n_kv_head, head_dim, cache.page_tokens, kind)
         floats = self.lib.mg_attention_shared_scratch_floats(*shape)
         scratch = table.new_empty((floats,)) if floats else None         # (words of 32 bits; few keys: one kernel, no scratch)

@@ -263,6 +263,14 @@ def test_attention_shared_through_paged_attention(ops, dtype):
     check_attention(case, ops.paged_attention(case.q, H, KV, D, D ** -0.5, case.cache, case.ctx), dtype)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("bounds", [(2 ** 31 - 1,) * 3, (2 ** 40, 2 ** 33, 2 ** 32), (1, 0, 2 ** 31 - 1)])
+def test_attention_shared_bounds_without_end(ops, dtype, bounds):
+    """Bounds beyond all numbers (no bounds, that is) count as what the block tables can hold."""
+    case = shared_case([(300, [90, 1, 5]), (40, [3, 1])], [200], (8, 2, 64), 16, dtype, seed=6, bounds=bounds, pad=1)
+    check_attention(case, run_attention(ops, case), dtype)
+
+
 @pytest.mark.parametrize("heads,rows,shared,page", [((8, 8, 96), 8, 300, 16), ((8, 8, 128), 5, 1000, 5), ((16, 8, 104), 4, 140, 64)])
 def test_attention_shared_many_short_ranges(ops, heads, rows, shared, page):
     """So many CTAs of few keys that they take the smallest rings: ranges of no, one and some keys, features padded to 128."""
