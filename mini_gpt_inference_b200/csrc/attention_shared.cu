@@ -13,6 +13,10 @@
 // cut into as many ranges as there are, of at least a fixed number of keys, so bounds that are too low cost time only.  The
 // same holds for the rows of a group.  A row that stands in front of the end of its group's shared tokens reads all its
 // keys for itself, and so does one that belongs to no group.
+//
+// A range without keys (their pages are missing) leaves m = -inf and l = 0.  One whose keys all score -inf leaves m = -inf and
+// l = 1: it counts for nothing beside others, and where there are no others the result is no number, as the softmax is.  Maxima
+// pass over a score that is no number; l does not, and neither does the result.
 #include <math.h>
 
 #include "blackwell.cuh"
@@ -162,13 +166,18 @@ __device__ __forceinline__ int pair_row(const SharedArgs& a, const Item& it, int
     return !it.shared || position_of(a, row) + 1 >= it.shared_keys ? row : -1;
 }
 
+// A row's result from its average, maximum and sum over all its keys (no key has a page: zeros).
+__device__ __forceinline__ float result_of(float v, float top, float sum) {
+    return sum == 0.f ? 0.f : top == -INFINITY ? NAN : v / sum;
+}
+
 // What a range leaves of feature d of a (row, head): the unnormalised average, with the maximum and the sum, or, where a row has one
 // range alone, the result.
 template <typename T>
 __device__ __forceinline__ void leave(const SharedArgs& a, const Item& it, int row, int head, int d, float v, float top, float sum) {
     const size_t pair = (size_t)row * a.n_head + head;
     if (a.direct) {
-        ((T*)a.out)[pair * a.D + d] = from_float<T>(sum != 0.f ? v / sum : 0.f);      // (no key has a page: zeros)
+        ((T*)a.out)[pair * a.D + d] = from_float<T>(result_of(v, top, sum));
         return;
     }
     const size_t at = pair * (a.shared_slots + a.own_slots) + it.slot;
@@ -217,6 +226,7 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_shared_simt_kernel(Sha
     extern __shared__ float4 smem4[];
     __shared__ int krow[BLOCK_KEYS], q_token[NQ], q_head[NQ];
     __shared__ float q_max[NQ], q_sum[NQ], q_corr[NQ];
+    __shared__ int seen;                                 // whether the range has a key
     constexpr int HALF = NQ / 2;
     const int tid = threadIdx.x, D = a.D, kv_head = blockIdx.y, share = a.n_head / a.n_kv_head;
     float* q_s = reinterpret_cast<float*>(smem4);        // [D][NQ]
@@ -236,6 +246,7 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_shared_simt_kernel(Sha
             q_head[tid] = kv_head * share + (q0 + tid) % share;
             q_max[tid] = -INFINITY;
             q_sum[tid] = 0.f;
+            seen = 0;
         }
         __syncthreads();
         for (int d = tid; d < D; d += SIMT_THREADS)
@@ -249,7 +260,10 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_shared_simt_kernel(Sha
             for (int j = 0; j < NQ; ++j) acc[i][j] = 0.f;
         for (int b0 = it.key0; b0 < it.key1; b0 += BLOCK_KEYS) {
             __syncthreads();
-            if (tid < BLOCK_KEYS) krow[tid] = cache_row(a, it, b0 + tid, kv_head);
+            if (tid < BLOCK_KEYS) {
+                krow[tid] = cache_row(a, it, b0 + tid, kv_head);
+                if (krow[tid] >= 0) seen = 1;
+            }
             __syncthreads();
             load_rows<T, VEC>((const T*)a.k_pages, krow, k_s, D + 1, D);
             load_rows<T, VEC>((const T*)a.v_pages, krow, v_s, D, D);
@@ -289,7 +303,7 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_shared_simt_kernel(Sha
                 float sum = 0.f;
 #pragma unroll
                 for (int k = 0; k < BLOCK_KEYS / 8; ++k) {
-                    const float e = top == -INFINITY ? 0.f : exp2f(x[k] - top);
+                    const float e = x[k] == -INFINITY ? 0.f : exp2f(x[k] - top);      // (no number stays none)
                     p_s[(k * 8 + part) * NQ + j] = e;
                     sum += e;
                 }
@@ -342,9 +356,10 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_shared_simt_kernel(Sha
 #pragma unroll
             for (int j = 0; j < NQ; ++j) {
                 if (q_token[j] < 0) continue;
+                const float sum = q_max[j] == -INFINITY && q_sum[j] == 0.f && seen ? 1.f : q_sum[j];
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    if (dl + i * SIMT_THREADS < D) leave<T>(a, it, q_token[j], q_head[j], dl + i * SIMT_THREADS, acc[i][j], q_max[j], q_sum[j]);
+                    if (dl + i * SIMT_THREADS < D) leave<T>(a, it, q_token[j], q_head[j], dl + i * SIMT_THREADS, acc[i][j], q_max[j], sum);
             }
     }
 }
@@ -499,12 +514,14 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaSizes<DP, NT, MANY>::CTAS) att
         // (j / 2) * 8 .., piece j % 2)
         const int krow = (lane & 7) + (((lane >> 3) & 1) << 3), kpiece = lane >> 4;
         const int vrow = (lane & 7) + (((lane >> 4) & 1) << 3), vpiece = (lane >> 3) & 1;
+        uint32_t seen = 0;                                              // whether this warp had a key
         for (int n = 0; n < my_units; ++n) {
             asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
             __syncwarp();                                               // this unit has landed
             const int next = row_of(n + STAGES + 1);
             const uint32_t k_at = mine_u + (uint32_t)(n % STAGES) * 2 * Z::TILE, v_at = k_at + Z::TILE;
             const uint32_t there = valid[warp][n % STAGES];
+            seen |= there;
             float s[NT][4];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
@@ -585,7 +602,7 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaSizes<DP, NT, MANY>::CTAS) att
                 }
                 if (g == 0) {
                     dst[DP] = ref[nt][i];
-                    dst[DP + 1] = sum[nt][i];
+                    dst[DP + 1] = ref[nt][i] == -INFINITY && sum[nt][i] == 0.f && seen ? 1.f : sum[nt][i];
                 }
             }
         __syncthreads();
@@ -599,7 +616,7 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaSizes<DP, NT, MANY>::CTAS) att
 #pragma unroll
             for (int w = 0; w < MMA_WARPS; ++w) {                       // warps in order
                 const float ref_w = part[(w * NT * 8 + tid) * PSTRIDE + DP];
-                const float f = ref_w == -INFINITY ? 0.f : exp2f(ref_w - top);
+                const float f = ref_w != -INFINITY ? exp2f(ref_w - top) : top == -INFINITY ? 1.f : 0.f;
                 weight[w][tid] = f;
                 l = fmaf(f, part[(w * NT * 8 + tid) * PSTRIDE + DP + 1], l);
             }
@@ -759,7 +776,7 @@ attention_shared_tc_kernel(SharedArgs a, const __grid_constant__ CUtensorMap map
             return w;
         };
         int n = 0, code = 0;                                            // blocks so far
-        bool holes = false, looked = false;                             // whether a page of the range is missing
+        bool holes = false, looked = false, seen = false;               // whether a page of the range is missing, one is there
         for (int q0 = first_pair, round = 0; q0 < pairs && code == 0; q0 += stride, ++round) {
             const int j0 = q0 + i * TC_PAIRS;
             if (j0 >= pairs) continue;                                  // no pairs for this tile
@@ -780,8 +797,13 @@ attention_shared_tc_kernel(SharedArgs a, const __grid_constant__ CUtensorMap map
             tc_fence_before();
             mbar_arrive(smem_u32(&sync.q_ready[i]));
             if (!looked) {                                              // (while the first keys are on their way)
-                for (int c = it.key0 / a.page_tokens + lane; c <= (it.key1 - 1) / a.page_tokens; c += 32) holes = holes || page_at(c) < 0;
+                for (int c = it.key0 / a.page_tokens + lane; c <= (it.key1 - 1) / a.page_tokens; c += 32) {
+                    const bool hole = page_at(c) < 0;
+                    holes = holes || hole;
+                    seen = seen || !hole;
+                }
                 holes = __any_sync(0xffffffffu, holes);
+                seen = __any_sync(0xffffffffu, seen);
                 looked = true;
             }
             float ref = -INFINITY, total = 0.f;
@@ -900,6 +922,7 @@ attention_shared_tc_kernel(SharedArgs a, const __grid_constant__ CUtensorMap map
                 }
             }
             total += other_half(total);
+            if (ref == -INFINITY && total == 0.f && seen) total = 1.f;
             if (write && h == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(ref, total);
             // (the queries' place is scratch no more)
             if (any_of(9 + i, 256, code != 0) && code == 0) code = 69;
@@ -1046,21 +1069,21 @@ __global__ void __launch_bounds__(128) attention_shared_join_kernel(SharedArgs a
         float high = top;
 #pragma unroll
         for (int u = 0; u < 8; ++u) high = fmaxf(high, ml[u].x);
-        const float corr = top == -INFINITY ? 0.f : exp2f(top - high);
+        const float corr = top == high ? 1.f : exp2f(top - high);
         top = high;
         total *= corr;
 #pragma unroll
         for (int j = 0; j < J; ++j) acc[j] *= corr;
 #pragma unroll
         for (int u = 0; u < 8; ++u) {                     // ranges in order
-            if (ml[u].x == -INFINITY) continue;
-            const float w = exp2f(ml[u].x - top);
+            if (ml[u].x == -INFINITY && ml[u].y == 0.f) continue;
+            const float w = top == -INFINITY ? 1.f : exp2f(ml[u].x - top);
             total = fmaf(w, ml[u].y, total);
 #pragma unroll
             for (int j = 0; j < J; ++j) acc[j] = fmaf(w, x[u][j], acc[j]);
         }
     }
-    const float inv = total != 0.f ? 1.0f / total : 0.f;  // (no key has a page: zeros)
+    const float inv = result_of(1.f, top, total);
 #pragma unroll
     for (int j = 0; j < J; ++j)
         if (lane + 32 * j < a.D) out[lane + 32 * j] = from_float<T>(acc[j] * inv);

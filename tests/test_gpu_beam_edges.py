@@ -1,0 +1,99 @@
+"""The beam search's kernels on inputs at the edge of what a call allows: numbers that are none, groups whose first rows see
+less than the others, scales below zero, large logits."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import plain_beam
+from test_gpu_beam import BF16, F32, check_choice, i32, run_attention, shared_case
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from mini_gpt_inference_b200.kernels.ops import default_ops
+
+    return default_ops("cuda:0")
+
+
+# ---- attention: the kernels that a call may take, by type and shape ------------------------------------
+JOINED, DIRECT = [(300, [90, 1, 70]), (5, [1])], [(70, [5, 20, 9]), (5, [1])]
+KERNELS = {
+    "32-bit": (F32, (4, 2, 64), JOINED), "32-bit, one launch": (F32, (4, 2, 64), DIRECT),
+    "32-bit, many ranges": (F32, (4, 2, 64), [(700, [200, 1])]),
+    "32-bit, odd heads": (F32, (3, 3, 7), JOINED),
+    "bfloat16": (BF16, (4, 2, 64), JOINED), "bfloat16, one launch": (BF16, (4, 2, 64), DIRECT),
+    "bfloat16, both halves of a weight": (BF16, (4, 2, 48), JOINED), "bfloat16, odd heads": (BF16, (3, 3, 7), JOINED),
+    "tiles of 64": (BF16, (8, 8, 64), [(300, [90, 1, 70] * 14), (5, [1])]),
+    "tiles of 128": (BF16, (32, 8, 128), [(300, [90, 1, 70] * 5), (5, [1])]),
+}
+
+
+def set_keys(case, rows, tokens, kv_head, feature, value):
+    """Feature of the keys of some tokens of some rows, in the pages and in what the plain form sees."""
+    page = case.cache.page_tokens
+    for r in rows:
+        table = case.ctx.block_tables[0][int(case.ctx.token_request[r])].tolist()
+        for t in tokens:
+            if t < case.k[r].shape[1]:
+                case.cache.k_pages[table[t // page], kv_head, t % page, feature] = value
+                case.k[r][kv_head, t, feature] = value
+
+
+def check_numbers(case, out, dtype, scale=None):
+    """No numbers exactly where the 64-bit softmax has none, the others as close as ever."""
+    H, KV, D = case.heads
+    some = False
+    for r, (k, v) in enumerate(zip(case.k, case.v)):
+        want, size = plain_beam.attention_row(case.q[r, : H * D].cpu().reshape(H, D), k, v, D ** -0.5 if scale is None else scale)
+        got = out[r].double().cpu().reshape(H, D)
+        assert torch.equal(torch.isnan(got), torch.isnan(want)), r
+        some = some or bool(torch.isnan(want).any())
+        # (see test_gpu_beam.check_attention)
+        tol = 20 * math.sqrt(D) * 2.0 ** -24 * size + 1e-6
+        if dtype == BF16:
+            tol = tol + 2.0 ** -8 * (size + want.abs())
+        there = ~torch.isnan(want)
+        assert ((got - want).abs() <= tol)[there].all(), (r, float((got - want)[there].abs().max()))
+    return some
+
+
+@pytest.mark.parametrize("what", ["query", "shared key", "shared keys", "own key", "low query", "high query", "low shared keys",
+                                  "low first key"])
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_attention_shared_keeps_what_is_no_number(ops, kernel, what):
+    """A query or a key that is none, one or a whole range of them; scores of minus infinity everywhere, or of a range alone (which then
+    counts for nothing), and infinite ones."""
+    dtype, heads, groups = KERNELS[kernel]
+    case = shared_case(groups, [40], heads, 16, dtype, seed=51, pad=1)
+    H, KV, D = heads
+    n, first = len(case.k), len(groups[0][1])
+    q = case.q.view(n + 1, -1)
+    group, everyone = range(first), range(n)
+    if what == "query":
+        q[1, 3] = math.nan
+    elif what == "shared key":
+        set_keys(case, group, [33], KV - 1, 5, math.nan)
+    elif what == "shared keys":
+        set_keys(case, group, range(64), 0, 5, math.nan)
+    elif what == "own key":
+        set_keys(case, [first - 1], [case.k[first - 1].shape[1] - 1], 0, 5, math.nan)
+    elif what in ("low query", "high query"):
+        q[1, 0] = -math.inf if what == "low query" else math.inf
+        case.cache.k_pages[:, 0, :, 0] = case.cache.k_pages[:, 0, :, 0].abs() + 1
+        for k in case.k:
+            k[0, :, 0] = k[0, :, 0].abs() + 1
+    else:
+        q[:n, : H * D: D] = q[:n, : H * D: D].abs() + 1                      # every head's first feature
+        for head in range(KV):
+            set_keys(case, group if what == "low shared keys" else everyone, range(64) if what == "low shared keys" else [0], head, 0, -math.inf)
+    out = run_attention(ops, case)
+    ops.check_status()
+    some = check_numbers(case, out, dtype)
+    assert some == (what not in ("low shared keys", "low first key"))
+    assert (out[n:] == 0).all()
