@@ -92,6 +92,19 @@ __device__ __forceinline__ int group_tokens(const SharedArgs& a, int row) {
     return tokens;
 }
 
+// The request of the first of a group's rows that sees all its shared tokens, whose block table leads to them all (a row in
+// front of their end, or one of padding, need not have their pages); -1: none does.  Whole warps call it.
+__device__ __forceinline__ int sharing_request(const SharedArgs& a, int first_row, int rows, int tokens) {
+    const int lane = threadIdx.x & 31;
+    for (int r0 = 0; r0 < rows; r0 += 32) {
+        const bool in = r0 + lane < rows;
+        const int request = in ? a.token_request[first_row + r0 + lane] : 0;      // (asked for together with the position)
+        const uint32_t found = __ballot_sync(0xffffffffu, in && position_of(a, first_row + r0 + lane) + 1 >= tokens);
+        if (found) return __shfl_sync(0xffffffffu, request, __ffs(found) - 1);
+    }
+    return -1;
+}
+
 // What a CTA works on: (row, head) pairs of `rows` rows and the keys key0 .. key1 - 1 that their ranges `slot` hold.
 struct Item {
     int first_row, rows, tile, tiles, key0, key1, slot, shared_keys;
@@ -118,7 +131,8 @@ __device__ __forceinline__ bool item_of(const SharedArgs& a, int item, Item& it)
         it.shared_keys = tokens_of(a, g);
         if (it.first_row < 0 || it.rows <= 0 || it.first_row >= a.n) return false;
         it.rows = min(it.rows, a.n - it.first_row);
-        request = a.token_request[it.first_row];
+        request = sharing_request(a, it.first_row, it.rows, it.shared_keys);
+        if (request < 0) return false;
         const int step = range_keys(it.shared_keys, a.shared_slots, a.shared_least);
         it.key0 = it.slot * step;
         it.key1 = min(it.shared_keys, it.key0 + step);
@@ -1257,8 +1271,8 @@ MG_API int mg_attention_shared_launches(int n_groups, int max_rows, int max_toke
 // Attention of n single query tokens, groups of which share their first keys.  q: rows of q_stride elements whose first
 // n_head * head_dim are the queries; pages [num_pages, n_kv_head, page_tokens, head_dim]; table [n_requests, max_pages]
 // (a page below zero or beyond the pool: its keys are not there); groups [n_groups, 3] ints on the device = (first row,
-// rows, shared tokens): rows of different groups are different ones, and the block tables of a group's rows lead to the
-// same keys and values over the shared tokens.  max_rows, max_tokens, max_behind: how many rows a group has, how many
+// rows, shared tokens): rows of different groups are different ones, and the block tables of those of a group's rows that
+// see all its shared tokens lead to the same keys and values over them.  max_rows, max_tokens, max_behind: how many rows a group has, how many
 // tokens it shares and how many keys a row has besides, at most (bounds that are too low cost time).  A row whose position
 // is below zero is padding: its output is zeros.  scratch: mg_attention_shared_scratch_floats() floats, 16-byte aligned,
 // that no other launch uses meanwhile.  kind: 0 32-bit, 1 bfloat16 with pages and rows of queries at 16-byte boundaries, 2 other

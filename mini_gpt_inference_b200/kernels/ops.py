@@ -966,8 +966,8 @@ class CudaOps:
         """``paged_attention`` for a step of single tokens, groups of which share their first tokens
         (``ctx.shared_prefix``, see ``SharedPrefix``): a group's common keys and values are read once.  Each row sees the
         keys 0 .. its position of its own request; a row in front of the end of its group's shared tokens, or of no group,
-        reads all of them for itself; one at a position below zero is padding, its result zeros.  Heads of up to 256
-        features; no window, no values in the key rows."""
+        reads all of them for itself (its block table need not lead to the others); one at a position below zero is padding, its
+        result zeros.  Heads of up to 256 features; no window, no values in the key rows."""
         shared = getattr(ctx, "shared_prefix", None)
         if shared is None:
             raise KernelLibraryError("attention (shared): the step names no groups of rows")

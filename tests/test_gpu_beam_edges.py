@@ -97,3 +97,30 @@ def test_attention_shared_keeps_what_is_no_number(ops, kernel, what):
     some = check_numbers(case, out, dtype)
     assert some == (what not in ("low shared keys", "low first key"))
     assert (out[n:] == 0).all()
+
+
+@pytest.mark.parametrize("how", ["short first rows", "padding first", "nobody sees all"])
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_attention_shared_takes_pages_of_a_row_that_sees_them(ops, kernel, how):
+    """Groups whose first rows stand in front of the shared end, with block tables as ``step_tables`` leaves them (nothing behind the
+    last page), or are padding, whose request is another one's."""
+    dtype, heads, groups = KERNELS[kernel]
+    shared, behind = groups[0]
+    short = [-shared + 1, -shared + 20] if how != "padding first" else []
+    behind = short + ([1 - shared // 2] * 5 if how == "nobody sees all" else behind)
+    case = shared_case([(shared, behind), *groups[1:]], [40], heads, 16, dtype, seed=61)
+    for r, k in enumerate(case.k):
+        request = int(case.ctx.token_request[r])
+        case.ctx.block_tables[0][request, -(-k.shape[1] // 16):] = -1
+    padding = []
+    if how == "padding first":
+        padding = [0, 1] if len(behind) > 3 else [0]
+        for r in padding:
+            case.ctx.positions[r] = -1
+            case.ctx.token_request[r] = int(case.ctx.token_request[len(case.k) - 1])
+    out = run_attention(ops, case)
+    ops.check_status()
+    assert (out[padding] == 0).all()
+    keep = [r for r in range(len(case.k)) if r not in padding]
+    case.k, case.v, case.q, out = [case.k[r] for r in keep], [case.v[r] for r in keep], case.q[keep], out[keep]
+    assert not check_numbers(case, out, dtype)
