@@ -1192,7 +1192,9 @@ int padded_head(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 2
 size_t sums_at(size_t slots, int head_dim) { return (slots * head_dim + 3) / 4 * 4; }
 
 // How a launch is cut.
-enum Kind { F32 = 0, BF16_ALIGNED = 1, BF16 = 2 };      // aligned: pages and rows of queries at 16-byte boundaries
+// (aligned: pages and rows of queries at 16-byte boundaries, and a scale above zero: the tiles take the largest score before they
+// scale it)
+enum Kind { F32 = 0, BF16_ALIGNED = 1, BF16 = 2 };
 struct Cut {
     bool direct;         // a range a row, no groups: one launch
     bool mma, tc;        // the warp-level tensor cores; shared ranges on tcgen05
@@ -1275,8 +1277,8 @@ MG_API int mg_attention_shared_launches(int n_groups, int max_rows, int max_toke
 // see all its shared tokens lead to the same keys and values over them.  max_rows, max_tokens, max_behind: how many rows a group has, how many
 // tokens it shares and how many keys a row has besides, at most (bounds that are too low cost time).  A row whose position
 // is below zero is padding: its output is zeros.  scratch: mg_attention_shared_scratch_floats() floats, 16-byte aligned,
-// that no other launch uses meanwhile.  kind: 0 32-bit, 1 bfloat16 with pages and rows of queries at 16-byte boundaries, 2 other
-// bfloat16.  status: a word that gets a code if a bounded wait runs out.  mg_attention_shared_launches()
+// that no other launch uses meanwhile.  kind: 0 32-bit, 1 bfloat16 with pages and rows of queries at 16-byte boundaries and a scale
+// above zero, 2 other bfloat16.  status: a word that gets a code if a bounded wait runs out.  mg_attention_shared_launches()
 // launches.  MG_ERR_UNSUPPORTED for heads of more than 256 features.
 MG_API int mg_attention_shared(const void* q, long long q_stride, const void* k_pages, const void* v_pages, const int* table,
                                const int* token_request, const int* positions, const int* groups, int n_groups, int max_rows,
@@ -1318,6 +1320,7 @@ MG_API int mg_attention_shared(const void* q, long long q_stride, const void* k_
     int rc;
     MG_REQUIRE(kind != BF16_ALIGNED || (q_stride % 8 == 0 && (((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages) & 15) == 0),
                "attention (shared): rows that are said to be 16-byte aligned and are not");
+    MG_REQUIRE(kind != BF16_ALIGNED || scale > 0.f, "attention (shared): a scale that is said to be above zero and is not");
     if (c.tc) {
         rc = head_dim == 64 ? launch_tc<64>(a, status, s) : launch_tc<128>(a, status, s);
         if (rc != MG_OK) return rc;

@@ -973,8 +973,9 @@ class CudaOps:
             raise KernelLibraryError("attention (shared): the step names no groups of rows")
         k, v, n = cache.k_pages, cache.v_pages, qkv.shape[0]
         self._want(qkv, k.dtype, "qkv", 2)
-        # 32-bit, bfloat16 at 16-byte boundaries, other bfloat16
-        kind = self._is_bf16(qkv) and (2 if qkv.shape[1] % 8 or (qkv.data_ptr() | k.data_ptr() | v.data_ptr()) % 16 else 1)
+        # 32-bit, bfloat16 at 16-byte boundaries and of a scale above zero, other bfloat16
+        plain = not ctypes.c_float(scale).value > 0 or qkv.shape[1] % 8 or (qkv.data_ptr() | k.data_ptr() | v.data_ptr()) % 16
+        kind = self._is_bf16(qkv) and (2 if plain else 1)
         table = self._want(ctx.block_tables[cache.group], torch.int32, "block_table", 2)
         groups = self._want(shared.groups, torch.int32, "groups of rows", 2)
         if self._want(v, k.dtype, "v_pages", 4).shape != self._want(k, None, "k_pages", 4).shape or (

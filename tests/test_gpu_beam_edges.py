@@ -124,3 +124,15 @@ def test_attention_shared_takes_pages_of_a_row_that_sees_them(ops, kernel, how):
     keep = [r for r in range(len(case.k)) if r not in padding]
     case.k, case.v, case.q, out = [case.k[r] for r in keep], [case.v[r] for r in keep], case.q[keep], out[keep]
     assert not check_numbers(case, out, dtype)
+
+
+@pytest.mark.parametrize("scale", [-0.2, 0.0])
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_attention_shared_scales_that_are_not_positive(ops, kernel, scale):
+    dtype, heads, groups = KERNELS[kernel]
+    case = shared_case(groups, [40], heads, 16, dtype, seed=62, pad=1)
+    H, KV, D = heads
+    out = ops.paged_attention_shared(case.q, H, KV, D, scale, case.cache, case.ctx)
+    ops.check_status()
+    assert not check_numbers(case, out, dtype, scale)
+    assert (out[len(case.k):] == 0).all()
