@@ -383,8 +383,9 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_shared_simt_kernel(Sha
 // that a row's own keys, read for one pair or a few, waste little.  A CTA's four warps take 16 keys in turn; each copies its
 // own rows from their pages (cp.async, a ring of stages), and keeps maximum, sum and average of its own, so the loop has no
 // barrier.  The maximum is a reference that moves only when a score is more than 2^REF_SLACK above it: then everything so
-// far is rescaled.  P goes into the product rounded to bfloat16 (2^-8 of a weight at most, as in the other attention
-// kernels of this type), the sums are of the 32-bit weights.
+// far is rescaled.  P goes into the product rounded to bfloat16 (2^-8 of a weight at most) for the heads whose weights the kernels of
+// unshared keys round so (16, 32, 64, 128 and 256 features); for the others, where those hold more, as two bfloat16 numbers (FULL:
+// 2^-16 of a weight).  The sums are of the 32-bit weights.
 constexpr float REF_SLACK = 8.f;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -414,6 +415,9 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
+// The 32-bit values of a pair's numbers.
+__device__ __forceinline__ float bf16_low(uint32_t p) { return __uint_as_float(p << 16); }
+__device__ __forceinline__ float bf16_high(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
 
 constexpr int MMA_THREADS = 128, MMA_WARPS = MMA_THREADS / 32, UNIT = 16;       // keys a warp takes at a time
 
@@ -429,7 +433,7 @@ struct MmaSizes {
     static constexpr size_t SMEM = (size_t)MMA_WARPS * STAGES * 2 * TILE;
 };
 
-template <int DP, int NT, bool MANY>      // NT: tiles of 8 pairs that a CTA takes at once
+template <int DP, int NT, bool MANY, bool FULL>      // NT: tiles of 8 pairs that a CTA takes at once
 __global__ void __launch_bounds__(MMA_THREADS, MmaSizes<DP, NT, MANY>::CTAS) attention_shared_mma_kernel(SharedArgs a) {
     using Z = MmaSizes<DP, NT, MANY>;
     constexpr int STAGES = Z::STAGES, CPR = DP / 8, ROWB = 2 * DP;
@@ -574,7 +578,7 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaSizes<DP, NT, MANY>::CTAS) att
                         }
                     }
             }
-            uint32_t pb[NT][2];
+            uint32_t pb[NT][2], rest[NT][2];                           // the weights, and what their rounding leaves
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float e[4];
@@ -583,8 +587,12 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaSizes<DP, NT, MANY>::CTAS) att
                     e[i] = exp2_approx(s[nt][i] - (ref[nt][i & 1] == -INFINITY ? 0.f : ref[nt][i & 1]));
                     sum[nt][i & 1] += e[i];
                 }
-                pb[nt][0] = movmatrix_trans(pack_bf16(e[0], e[1]));
-                pb[nt][1] = movmatrix_trans(pack_bf16(e[2], e[3]));
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t p = pack_bf16(e[2 * h], e[2 * h + 1]);
+                    pb[nt][h] = movmatrix_trans(p);
+                    if constexpr (FULL) rest[nt][h] = movmatrix_trans(pack_bf16(e[2 * h] - bf16_low(p), e[2 * h + 1] - bf16_high(p)));
+                }
             }
 #pragma unroll
             for (int dm = 0; dm < DP / 16; ++dm) {
@@ -592,7 +600,10 @@ __global__ void __launch_bounds__(MMA_THREADS, MmaSizes<DP, NT, MANY>::CTAS) att
                 ldmatrix_x4_trans(f, v_at + vrow * ROWB + (((dm * 2 + vpiece) ^ ((vrow / RPL) % SWZ)) * 16));
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
-                    if (nt < nts) mma_bf16(o[nt][dm], f, pb[nt][0], pb[nt][1]);
+                    if (nt < nts) {
+                        mma_bf16(o[nt][dm], f, pb[nt][0], pb[nt][1]);
+                        if constexpr (FULL) mma_bf16(o[nt][dm], f, rest[nt][0], rest[nt][1]);
+                    }
             }
             __syncwarp();                                               // the unit is used up
             load(n + STAGES, row);
@@ -1170,9 +1181,13 @@ int launch_simt(const SharedArgs& a, int pairs, cudaStream_t s) {
 
 constexpr int DIRECT_KEYS = 256, DIRECT_ROWS = 256, TC_LEAST_PAIRS = 32, TC_CTA_KEYS = 1000;
 
+// Head sizes that the kernels of unshared keys take with weights of bfloat16 (attention_decode.cu); others: see FULL.
+bool rounded_weights(int d) { return d == 16 || d == 32 || d == 64 || d == 128 || d == 256; }
+
 template <int DP, int NT, bool MANY>
 int launch_mma_tiles(const SharedArgs& a, cudaStream_t s) {
-    return launch_ranges(attention_shared_mma_kernel<DP, NT, MANY>, MMA_THREADS, MmaSizes<DP, NT, MANY>::SMEM, a, s);
+    return launch_ranges(rounded_weights(a.D) ? attention_shared_mma_kernel<DP, NT, MANY, false> : attention_shared_mma_kernel<DP, NT, MANY, true>,
+                         MMA_THREADS, MmaSizes<DP, NT, MANY>::SMEM, a, s);
 }
 template <int DP>
 int launch_mma(const SharedArgs& a, int pair_tiles, bool many, cudaStream_t s) {

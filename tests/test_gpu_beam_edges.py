@@ -136,3 +136,20 @@ def test_attention_shared_scales_that_are_not_positive(ops, kernel, scale):
     ops.check_status()
     assert not check_numbers(case, out, dtype, scale)
     assert (out[len(case.k):] == 0).all()
+
+
+@pytest.mark.parametrize("heads,page", [((8, 2, 40), 16), ((4, 4, 8), 8), ((4, 2, 48), 5), ((12, 4, 104), 16), ((6, 1, 120), 64), ((3, 3, 136), 16), ((8, 2, 200), 32)])
+@pytest.mark.parametrize("shape", [[(300, [90, 1, 70]), (5, [1])], [(70, [5, 20, 9])], [(1000, [3] * 24)]])
+def test_attention_shared_holds_weights_as_paged_attention_does(ops, heads, page, shape):
+    """Heads whose softmax weights ``paged_attention`` holds in more than bfloat16's 8 bits: so do these, and what a result is off by is
+    its own rounding."""
+    case = shared_case(shape, [40], heads, page, BF16, seed=63)
+    H, KV, D = heads
+    out = run_attention(ops, case)
+    for r, (k, v) in enumerate(zip(case.k, case.v)):
+        want, size = plain_beam.attention_row(case.q[r, : H * D].cpu().reshape(H, D), k, v, D ** -0.5)
+        # a weight as two bfloat16 numbers: half a step of half a step, 2^-16 of it; 32-bit sums (see check_attention); half a step of
+        # the result
+        tol = (2.0 ** -16 + 20 * math.sqrt(D) * 2.0 ** -24) * size + 2.0 ** -8 * want.abs() + 1e-6
+        bad = (out[r].double().cpu().reshape(H, D) - want).abs() / tol
+        assert (bad <= 1).all(), (r, float(bad.max()))
