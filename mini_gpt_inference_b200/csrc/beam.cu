@@ -142,10 +142,11 @@ beam_rows_kernel(const float* __restrict__ logits, const int* __restrict__ ended
             sum *= exp2f((top - high) * log2e);
             top = high;
         }
-        const float shift = top == -INFINITY ? 0.f : top * log2e;
+        // (first the difference, then log2 e: what is rounded does not grow with the logits, and the largest one counts as 1)
+        const float base = top == -INFINITY ? 0.f : top;
         float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < 16; ++e) part[e & 3] += exp2_approx(fmaf(x[e], log2e, -shift));
+        for (int e = 0; e < 16; ++e) part[e & 3] += exp2_approx((x[e] - base) * log2e);
         sum += (part[0] + part[1]) + (part[2] + part[3]);
     }
     const float warp_top = warp_max(top);

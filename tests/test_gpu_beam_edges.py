@@ -153,3 +153,23 @@ def test_attention_shared_holds_weights_as_paged_attention_does(ops, heads, page
         tol = (2.0 ** -16 + 20 * math.sqrt(D) * 2.0 ** -24) * size + 2.0 ** -8 * want.abs() + 1e-6
         bad = (out[r].double().cpu().reshape(H, D) - want).abs() / tol
         assert (bad <= 1).all(), (r, float(bad.max()))
+
+
+# ---- the choice of the next beams ------------------------------------------------------------------------
+@pytest.mark.parametrize("offset", [-10000.0, -1000.0, 100.0, 1000.0, 10000.0])
+@pytest.mark.parametrize("certain", [False, True])
+@pytest.mark.parametrize("rows", [(2, 3), (8, 16)])
+def test_beam_select_of_large_logits(ops, rows, offset, certain):
+    """A number added to all logits of a row changes no score, and no log probability is above zero."""
+    gen = torch.Generator().manual_seed(7)
+    groups, beams = rows
+    vocab = 5000
+    logits = torch.randn(groups * beams, vocab, generator=gen) * 2 + offset + torch.rand(groups * beams, 1, generator=gen)
+    if certain:
+        logits[torch.arange(groups * beams), torch.randint(0, vocab, (groups * beams,), generator=gen)] += 40.0
+    scores = -3 * torch.rand(groups, beams, generator=gen)
+    got = ops.beam_select(logits.cuda(), scores.cuda(), beams)
+    want = plain_beam.beam_select(logits, scores, beams)
+    check_choice(got, want, groups, beams)                                 # (its tolerance knows nothing of the offset)
+    parents = got.parents.long().cpu()
+    assert (got.scores.cpu().reshape(-1) <= scores.reshape(-1)[parents]).all()
