@@ -31,7 +31,7 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--top-p", type=float, default=None)
     ap.add_argument("--seed", type=int, default=None)
     ap.add_argument("--beams", type=int, default=None, help="search for the best continuations with so many beams, in place of sampling")
-    ap.add_argument("--length-penalty", type=float, default=0.0, help="with --beams: rank by the log probability over length to this power")
+    ap.add_argument("--length-penalty", type=float, default=0.0, help="with --beams: rank by the log probability over length to this power (-16 to 16)")
     ap.add_argument("--eot-id", type=int, default=None, help="with --beams: the token id that ends a continuation")
     ap.add_argument("--vocab-limit", type=int, default=None,
                     help="ids at and above this are never sampled: rows that only pad the embedding "

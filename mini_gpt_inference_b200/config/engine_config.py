@@ -12,7 +12,6 @@ unlike the reference, ``seed`` is honoured (per-request counter-based RNG).
 
 from __future__ import annotations
 
-import math
 from dataclasses import dataclass, field
 
 
@@ -54,10 +53,13 @@ def canonical_dtype(name: str) -> str:
     return table[key]
 
 
+MAX_LENGTH_PENALTY = 16.0      # either way: any length below 2^31 to that power, and a log probability over it, fits 64 bits
+
+
 @dataclass
 class BeamParams:
     """A beam search: the ``beams`` best continuations at every step, ranked by the sum of their tokens' log probabilities over
-    ``length ** length_penalty``."""
+    ``length ** length_penalty`` (-16 to 16)."""
 
     beams: int = 4
     max_tokens: int = 128
@@ -68,8 +70,8 @@ class BeamParams:
             raise ValueError("beams must be 1 to 32")
         if self.max_tokens <= 0:
             raise ValueError("max_tokens must be positive")
-        if not math.isfinite(self.length_penalty):
-            raise ValueError("length_penalty must be a finite number")
+        if not -MAX_LENGTH_PENALTY <= self.length_penalty <= MAX_LENGTH_PENALTY:
+            raise ValueError(f"length_penalty must be a number from {-MAX_LENGTH_PENALTY:g} to {MAX_LENGTH_PENALTY:g}")
 
 
 @dataclass

@@ -9,12 +9,12 @@ computes anything on this path.
 from __future__ import annotations
 
 import ctypes
-import math
 import weakref
 from dataclasses import dataclass
 
 import torch
 
+from ..config.engine_config import MAX_LENGTH_PENALTY
 from . import library
 from .attention_plan import KEY_CHUNK, query_tiles
 from .library import KernelLibraryError, check
@@ -1848,8 +1848,8 @@ class CudaOps:
         """The best ``beams`` continuations of every group of rows.  ``scores`` (32-bit ``[groups, in_beams]``, ``in_beams`` from 1
         to ``beams``): the sums of the rows' log probabilities so far; ``logits`` (32-bit ``[groups * in_beams, vocab]``).  A
         continuation of row ``b`` by id ``t`` is worth ``score_b + log_softmax(logits_b)_t`` and ranked by that over
-        ``length ** length_penalty``, its length being ``lengths[b] + 1`` (int32 per row; without a penalty they may be left
-        out).  Equal ranks go to the lower row, in a row to the larger logit and then the lower id; a logit or a value that is
+        ``length ** length_penalty`` (-16 to 16), its length being ``lengths[b] + 1`` (int32 per row; without a penalty they may be
+        left out).  Equal ranks go to the lower row, in a row to the larger logit and then the lower id; a logit or a value that is
         no number counts as minus infinity.  A row that has ``ended`` (int32, not 0) has one continuation, itself, by
         ``end_token``.  ``vocab_limit``: ids at or above it do not exist.
 
@@ -1868,8 +1868,8 @@ class CudaOps:
             if t is not None and self._want(t, torch.int32, name, 1).numel() != rows:
                 raise KernelLibraryError(f"beam_select: {name} does not match the rows")
         length_penalty = float(length_penalty)
-        if not math.isfinite(length_penalty) or (length_penalty and lengths is None):
-            raise KernelLibraryError("beam_select: a length penalty that is no number, or without lengths")
+        if not -MAX_LENGTH_PENALTY <= length_penalty <= MAX_LENGTH_PENALTY or (length_penalty and lengths is None):
+            raise KernelLibraryError(f"beam_select: a length penalty beyond {MAX_LENGTH_PENALTY:g}, or without lengths")
         if end_token is None and ended is not None:
             raise KernelLibraryError("beam_select: ended beams without an end_token")
         if end_token is not None and not 0 <= int(end_token) < limit:
