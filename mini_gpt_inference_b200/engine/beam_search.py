@@ -25,7 +25,7 @@ from ..cache.manager import NO_PAGE, CacheFullError
 from ..config.engine_config import BeamParams
 from ..kernels.ops import BeamChoice
 from ..parts.context import SharedPrefix, StepContext
-from .runner import ModelRunner, StepEntry, _no_collection
+from .runner import ModelRunner, StepEntry, StepError, _no_collection
 
 
 def _bucket(n: int, most: int) -> int:
@@ -225,5 +225,7 @@ class BeamSearch:
                 mine.append({"token_ids": ids[::-1][: lengths[row]], "logprob": scores[row],
                              "score": scores[row] / max(1, lengths[row]) ** params.length_penalty,
                              "finish_reason": "eot" if ended[row] else "length"})
+            if not mine:
+                raise StepError(f"prompt {g}: no continuation has a log probability (the model's logits are infinite or no numbers)")
             found.append(mine)
         return found

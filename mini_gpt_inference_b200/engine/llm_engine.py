@@ -322,7 +322,9 @@ class LLMEngine:
         the device; requests that the engine holds wait meanwhile and keep their caches.  Returns, in the order of the prompts,
         up to ``beams`` dicts, the best first, with ``token_ids`` (generated only, an end of text included), ``logprob`` (the sum
         of their log probabilities), ``score`` (what they are ranked by) and ``finish_reason`` (``"eot"`` or ``"length"``).
-        Raises ``CacheFullError`` where the pools do not hold ``beams`` requests per prompt (beams share their prompt's pages)."""
+        Raises ``CacheFullError`` where the pools do not hold ``beams`` requests per prompt (beams share their prompt's pages; layers
+        with a window hold the pages of a whole continuation too, until the search ends), and ``StepError`` where no continuation of
+        a prompt has a log probability (logits that are infinite or no numbers; a beam whose logits become so is dropped)."""
         params = params or BeamParams()
         for i, prompt in enumerate(prompts):
             if len(prompt) == 0:

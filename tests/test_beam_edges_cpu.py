@@ -12,6 +12,7 @@ from test_beam_cpu import ops  # noqa: F401
 from test_beam_search_cpu import engine_for
 
 from mini_gpt_inference_b200 import BeamParams
+from mini_gpt_inference_b200.engine.runner import StepError
 from mini_gpt_inference_b200.kernels.library import KernelLibraryError
 
 
@@ -35,3 +36,28 @@ def test_length_penalties_beyond_the_bound_are_refused(ops, penalty):  # noqa: F
     logits, lengths = torch.zeros(6, 50), torch.zeros(6, dtype=torch.int32)
     with pytest.raises(KernelLibraryError, match="length penalty"):
         ops.beam_select(logits, torch.zeros(2, 3), 3, lengths=lengths, length_penalty=penalty)
+
+
+@pytest.mark.parametrize("value", [math.nan, -math.inf, math.inf])
+def test_a_model_without_log_probabilities_is_told(value, monkeypatch):
+    """A prompt none of whose continuations has a log probability is an error, not a prompt without continuations; nothing stays
+    behind, and the next search is as ever."""
+    engine, last, tokens, vocab = engine_for("A")
+    prompts = [tokens(9, 3), tokens(5, 4)]
+    forward = engine.runner._forward
+
+    def broken(ctx):
+        logits = forward(ctx)
+        if logits is not None:
+            logits[-1] = value
+        return logits
+
+    monkeypatch.setattr(engine.runner, "_forward", broken)
+    with pytest.raises(StepError, match="prompt 1"):
+        engine.beam_search(prompts, BeamParams(beams=3, max_tokens=1))
+    with pytest.raises(StepError, match="prompt 0"):
+        engine.beam_search(prompts[:1], BeamParams(beams=1, max_tokens=4))
+    assert engine.stats()["allocated_blocks"] == 0
+    monkeypatch.setattr(engine.runner, "_forward", forward)
+    found = engine.beam_search(prompts[:1], BeamParams(beams=3, max_tokens=4))[0]
+    assert [h["token_ids"] for h in found] == [ids for ids, _, _ in plain_beam.search(last, prompts[0], 3, 4)]
