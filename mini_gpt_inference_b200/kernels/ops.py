@@ -112,6 +112,12 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _span(t):
+    """The addresses of a contiguous tensor's numbers: first, and one behind the last."""
+    at = t.data_ptr()
+    return at, at + t.numel() * t.element_size()
+
+
 def _numbers(values):
     return (ctypes.c_longlong * len(values))(*values)
 
@@ -1887,6 +1893,13 @@ class CudaOps:
                     raise KernelLibraryError(f"beam_select: no room for {name}")
             if tuple(self._want(out.scores, torch.float32, "scores", 2).shape) != (groups, beams):
                 raise KernelLibraryError("beam_select: no room for scores")
+            # (a group's rows are read before they are written, another group's need not be)
+            inputs = [_span(t) for t in (logits, scores, ended, lengths) if t is not None]
+            outputs = [_span(t) for t in (out.tokens, out.parents, out.scores, out.ranks, out.ended, out.lengths) if t is not None]
+            for i, (at, end_at) in enumerate(outputs):
+                if any(at < b and a < end_at and not ((a, b) == (at, end_at) and in_beams == beams) for a, b in inputs) or any(
+                        at < b and a < end_at for a, b in outputs[:i]):
+                    raise KernelLibraryError("beam_select: outputs that share memory with one another or, but for the same rows, with the inputs")
         if n == 0:
             return out
         scratch = logits.new_empty((self.lib.mg_beam_select_scratch_bytes(groups, in_beams, beams, limit) // 4,))

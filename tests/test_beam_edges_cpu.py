@@ -14,6 +14,7 @@ from test_beam_search_cpu import engine_for
 from mini_gpt_inference_b200 import BeamParams
 from mini_gpt_inference_b200.engine.runner import StepError
 from mini_gpt_inference_b200.kernels.library import KernelLibraryError
+from mini_gpt_inference_b200.kernels.ops import BeamChoice
 
 
 @pytest.mark.parametrize("penalty", [-16.0, -3.5, 16.0])
@@ -61,3 +62,37 @@ def test_a_model_without_log_probabilities_is_told(value, monkeypatch):
     monkeypatch.setattr(engine.runner, "_forward", forward)
     found = engine.beam_search(prompts[:1], BeamParams(beams=3, max_tokens=4))[0]
     assert [h["token_ids"] for h in found] == [ids for ids, _, _ in plain_beam.search(last, prompts[0], 3, 4)]
+
+
+def test_outputs_of_a_choice_that_lie_in_its_inputs_are_refused(ops):  # noqa: F811
+    """In place only where rows stay rows: as many beams before as after, and the same tensor, not a part of it."""
+    i32 = lambda n: torch.zeros(n, dtype=torch.int32)  # noqa: E731
+
+    def call(beams, in_beams, replace):
+        scores, ended, lengths = torch.zeros(2, in_beams), i32(2 * in_beams), i32(2 * in_beams)
+        logits, big = torch.zeros(2 * in_beams, 50), i32(100)
+        given = dict(scores=scores, ended=ended, lengths=lengths, logits=logits.view(torch.int32).reshape(-1), big=big)
+        n = 2 * beams
+        out = dict(tokens=i32(n), parents=i32(n), scores=torch.zeros(2, beams), ranks=i32(n), ended=i32(n), lengths=i32(n))
+        out.update(replace(given, n))
+        ops.beam_select(logits, scores, beams, ended=ended, lengths=lengths, end_token=1, out=BeamChoice(**out))
+
+    bad = [
+        (4, 2, lambda g, n: dict(tokens=g["logits"][:n])),
+        (3, 3, lambda g, n: dict(parents=g["logits"][4:4 + n])),
+        (3, 3, lambda g, n: dict(tokens=g["big"][:n], parents=g["big"][2:2 + n])),
+        (3, 3, lambda g, n: dict(tokens=g["big"][:n], ranks=g["big"][:n])),
+        (3, 3, lambda g, n: dict(tokens=g["lengths"], parents=g["lengths"])),
+    ]
+    for beams, in_beams, replace in bad:
+        with pytest.raises(KernelLibraryError, match="memory"):
+            call(beams, in_beams, replace)
+    # views that overlap an input by a part, and an input of other rows: one allocation for both
+    for beams, in_beams, shift in ((3, 3, 1), (3, 3, -1), (4, 2, 0)):
+        both = i32(64)
+        ended, lengths = both[8: 8 + 2 * in_beams], i32(2 * in_beams)
+        out = BeamChoice(i32(2 * beams), i32(2 * beams), torch.zeros(2, beams), i32(2 * beams), both[8 + shift: 8 + shift + 2 * beams], i32(2 * beams))
+        with pytest.raises(KernelLibraryError, match="memory"):
+            ops.beam_select(torch.zeros(2 * in_beams, 50), torch.zeros(2, in_beams), beams, ended=ended, lengths=lengths, end_token=1, out=out)
+    with pytest.raises(AssertionError, match="mg_beam_select was reached"):      # in place: as the search calls it
+        call(3, 3, lambda g, n: dict(scores=g["scores"], ended=g["ended"], lengths=g["lengths"]))
