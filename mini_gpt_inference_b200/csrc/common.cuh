@@ -193,10 +193,16 @@ __device__ __forceinline__ float gelu_exp(float u) {
 // may start.  Both are no-ops when the launch carries no such dependency.  The host switch
 // mg_set_dependent_launch() turns the launch attribute on (used while a decode step is captured
 // into a CUDA graph, where every predecessor is a kernel).
+//
+// A step's integers (positions, requests, cache rows, block tables, rows of logits) are read in front of the wait too, by
+// projections, norms and attention: nothing that a kernel behind them may overlap writes them.  Either they were copied to the
+// device before the graph starts, or step_tables wrote them, which calls mg_next_launch_waits(): the kernel behind it is then
+// launched without the attribute, starts once step_tables has ended, and stands between it and all that follow.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-int mg_dependent_launch_enabled();
+int mg_take_dependent_launch();         // whether a kernel that is about to be launched may overlap the one in front of it
+void mg_next_launch_waits();
 
 template <typename... KArgs, typename... Args>
 static inline cudaError_t mg_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
@@ -207,7 +213,7 @@ static inline cudaError_t mg_launch(void (*kernel)(KArgs...), dim3 grid, dim3 bl
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
-    if (dependent && mg_dependent_launch_enabled()) {
+    if (mg_take_dependent_launch() && dependent) {
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr;

@@ -48,12 +48,13 @@ MG_API int mg_embed(const int* ids, const int* pos, const void* tok, const void*
     MG_REQUIRE(source == nullptr || previous != nullptr, "embed: token sources without the ids they point to");
     cudaStream_t s = (cudaStream_t)stream;
     int threads = width >= 256 ? 256 : 128;
-    if (weights_bf16)
-        embed_kernel<bf16><<<n_tokens, threads, 0, s>>>(ids, pos, (const bf16*)tok, (const bf16*)ptab, out, width, source,
-                                                       previous, vocab, n_positions, n_previous, scale);
-    else
-        embed_kernel<float><<<n_tokens, threads, 0, s>>>(ids, pos, (const float*)tok, (const float*)ptab, out, width,
-                                                        source, previous, vocab, n_positions, n_previous, scale);
+    // (never overlapping what is in front of it, which may have written the step's integers)
+    const cudaError_t e = weights_bf16
+        ? mg_launch(embed_kernel<bf16>, dim3(n_tokens), dim3(threads), 0, s, false, ids, pos, (const bf16*)tok, (const bf16*)ptab, out,
+                    width, source, previous, vocab, n_positions, n_previous, scale)
+        : mg_launch(embed_kernel<float>, dim3(n_tokens), dim3(threads), 0, s, false, ids, pos, (const float*)tok, (const float*)ptab, out,
+                    width, source, previous, vocab, n_positions, n_previous, scale);
+    if (e != cudaSuccess) return mg_set_error(MG_ERR_CUDA, "embed: %s", cudaGetErrorString(e));
     MG_CHECK_LAUNCH("embed");
     return MG_OK;
 }
@@ -135,16 +136,15 @@ MG_API int mg_embed_pairs(const int* ids, const int* pos, const int* token_reque
     MG_REQUIRE(source == nullptr || previous != nullptr, "embed_pairs: token sources without the ids they point to");
     cudaStream_t s = (cudaStream_t)stream;
     const int threads = width >= 256 ? 256 : 128;
-    if (weights_bf16)
-        embed_pairs_kernel<bf16><<<n_tokens, threads, 0, s>>>(
-            ids, pos, token_request, req_q_start, req_q_len, req_ctx_before, req_state_slot, (const bf16*)tok,
-            (const bf16*)pair, (const bf16*)ptab, out, state, state_stride, width, source, previous, vocab, n_positions,
-            n_previous, buckets, mul_prev, mul_cur, n_requests, n_slots, n_tokens);
-    else
-        embed_pairs_kernel<float><<<n_tokens, threads, 0, s>>>(
-            ids, pos, token_request, req_q_start, req_q_len, req_ctx_before, req_state_slot, (const float*)tok,
-            (const float*)pair, (const float*)ptab, out, state, state_stride, width, source, previous, vocab, n_positions,
-            n_previous, buckets, mul_prev, mul_cur, n_requests, n_slots, n_tokens);
+    // (as mg_embed: never overlapping what is in front of it)
+    const cudaError_t e = weights_bf16
+        ? mg_launch(embed_pairs_kernel<bf16>, dim3(n_tokens), dim3(threads), 0, s, false, ids, pos, token_request, req_q_start, req_q_len,
+                    req_ctx_before, req_state_slot, (const bf16*)tok, (const bf16*)pair, (const bf16*)ptab, out, state, state_stride,
+                    width, source, previous, vocab, n_positions, n_previous, buckets, mul_prev, mul_cur, n_requests, n_slots, n_tokens)
+        : mg_launch(embed_pairs_kernel<float>, dim3(n_tokens), dim3(threads), 0, s, false, ids, pos, token_request, req_q_start, req_q_len,
+                    req_ctx_before, req_state_slot, (const float*)tok, (const float*)pair, (const float*)ptab, out, state, state_stride,
+                    width, source, previous, vocab, n_positions, n_previous, buckets, mul_prev, mul_cur, n_requests, n_slots, n_tokens);
+    if (e != cudaSuccess) return mg_set_error(MG_ERR_CUDA, "embed_pairs: %s", cudaGetErrorString(e));
     MG_CHECK_LAUNCH("embed_pairs");
     return MG_OK;
 }

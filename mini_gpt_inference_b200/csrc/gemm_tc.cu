@@ -584,7 +584,7 @@ int launch(const void* a, const void* b, GemmArgs g, cudaStream_t s, const Exten
         attr[n_attr].val.clusterDim.y = attr[n_attr].val.clusterDim.z = 1;
         ++n_attr;
     }
-    if (mg_dependent_launch_enabled()) {
+    if (mg_take_dependent_launch()) {
         attr[n_attr].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[n_attr].val.programmaticStreamSerializationAllowed = 1;
         ++n_attr;

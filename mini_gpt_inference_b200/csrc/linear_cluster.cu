@@ -250,7 +250,7 @@ MG_API int mg_linear_cluster(const void* x, const void* w, const float* bias, vo
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.numAttrs = 1;
-    if (mg_dependent_launch_enabled()) {
+    if (mg_take_dependent_launch()) {
         attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[1].val.programmaticStreamSerializationAllowed = 1;
         cfg.numAttrs = 2;

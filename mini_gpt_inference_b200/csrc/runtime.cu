@@ -31,13 +31,19 @@ MG_API int mg_set_device(int device) {
     return MG_OK;
 }
 
-static int g_dependent_launch = 0;
+static int g_dependent_launch = 0, g_next_waits = 0;
 
-int mg_dependent_launch_enabled() { return g_dependent_launch; }
+int mg_take_dependent_launch() {
+    const int may = g_dependent_launch && !g_next_waits;
+    g_next_waits = 0;
+    return may;
+}
+void mg_next_launch_waits() { g_next_waits = 1; }
 
 // Turn programmatic dependent launch on (1) or off (0) for the kernels that support it.
 MG_API int mg_set_dependent_launch(int on) {
     g_dependent_launch = on ? 1 : 0;
+    g_next_waits = 0;
     return MG_OK;
 }
 

@@ -40,8 +40,7 @@ __global__ void __launch_bounds__(THREADS) step_tables_kernel(const __grid_const
     extern __shared__ int starts[];                      // [requests + 1]
     __shared__ int warp_total[THREADS / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    pdl_trigger();
-    pdl_wait();
+    pdl_wait();                                          // (nothing overlaps its end: see mg_next_launch_waits)
     // starts: each thread sums a run of requests, the runs' sums are scanned over the CTA
     const int per = (a.n_requests + THREADS - 1) / THREADS, r0 = min(a.n_requests, tid * per), r1 = min(a.n_requests, r0 + per);
     int sum = 0;
@@ -134,5 +133,6 @@ MG_API int mg_step_tables(const int* rows, const int* before, const int* fresh, 
                                     true, a);
     if (e != cudaSuccess) return mg_set_error(MG_ERR_CUDA, "step_tables: %s", cudaGetErrorString(e));
     MG_CHECK_LAUNCH("step_tables");
+    mg_next_launch_waits();                              // (kernels read these integers before they wait for what is in front of them)
     return MG_OK;
 }

@@ -4,6 +4,7 @@ less than the others, scales below zero, large logits."""
 from __future__ import annotations
 
 import math
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -173,3 +174,46 @@ def test_beam_select_of_large_logits(ops, rows, offset, certain):
     check_choice(got, want, groups, beams)                                 # (its tolerance knows nothing of the offset)
     parents = got.parents.long().cpu()
     assert (got.scores.cpu().reshape(-1) <= scores.reshape(-1)[parents]).all()
+
+
+# ---- a step's integers, where kernels overlap -------------------------------------------------------------
+@pytest.mark.parametrize("R", [3, 700])
+def test_step_tables_are_whole_before_what_reads_them(ops, R):
+    """Captured with overlapping launches, attention directly behind the step's integers (which it reads before it waits for what is in
+    front of it): every replay sees those of its own lengths."""
+    H, D, page, width = 4, 64, 16, 12
+    gen = torch.Generator().manual_seed(R)
+    pool = torch.randperm(R * width, generator=gen).to(torch.int32).reshape(R, width).cuda()
+    k, v = (torch.randn(R * width, H, page, D, generator=gen).to(BF16).cuda() for _ in range(2))
+    q = torch.randn(R, 3 * H * D, generator=gen).to(BF16).cuda()
+    before, ones = i32([5] * R), torch.ones(R, dtype=torch.int32, device="cuda")
+    cache = SimpleNamespace(k_pages=k, v_pages=v, group=0, page_tokens=page, window=None, writes=False, values_in_keys=False, keep_first=0)
+
+    def step():
+        t = ops.step_tables([pool], [page], before, ones, R)
+        ctx = SimpleNamespace(block_tables=t.block_tables, token_request=t.token_request, positions=t.positions, decode_only=True,
+                              extra={}, max_ctx_after=page * width)
+        return ops.paged_attention(q, H, H, D, D ** -0.5, cache, ctx)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    ops.set_dependent_launch(True)
+    try:
+        with torch.cuda.graph(graph):
+            out = step()
+    finally:
+        ops.set_dependent_launch(False)
+    for seed in range(4):
+        lengths = torch.randint(0, page * width - 1, (R,), generator=torch.Generator().manual_seed(seed)).to(torch.int32)
+        before.copy_(lengths)
+        graph.replay()
+        torch.cuda.synchronize()
+        for r in range(0, R, max(1, R // 40)):
+            n = int(lengths[r]) + 1
+            pages = pool[r, : -(-n // page)].long()
+            mine = [x[pages].transpose(0, 1).reshape(H, -1, D)[:, :n].cpu() for x in (k, v)]
+            want, size = plain_beam.attention_row(q[r, : H * D].cpu().reshape(H, D), *mine, D ** -0.5)
+            # (see test_gpu_beam.check_attention)
+            tol = 20 * math.sqrt(D) * 2.0 ** -24 * size + 1e-6 + 2.0 ** -8 * (size + want.abs())
+            assert ((out[r].double().cpu().reshape(H, D) - want).abs() <= tol).all(), (seed, r)
