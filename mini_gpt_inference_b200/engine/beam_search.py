@@ -187,8 +187,10 @@ class BeamSearch:
         longest = _bucket(longest_prompt + params.max_tokens, runner.max_context)
         key = (len(prompt_lengths), params.beams, _bucket(longest_prompt, runner.max_context), longest,
                _bucket(params.max_tokens, runner.max_context), params.length_penalty, end, vocab_limit)
-        step = self._steps.pop(key, None) or _Step(runner, *key)
-        capture = runner.use_cuda_graphs and params.max_tokens >= self.GRAPH_TOKENS
+        step = self._steps.pop(key, None)
+        # (one that is captured already serves any search)
+        capture = step is not None or (runner.use_cuda_graphs and params.max_tokens >= self.GRAPH_TOKENS)
+        step = step or _Step(runner, *key)
         if capture:
             while len(self._steps) >= self.GRAPHS:
                 self._steps.pop(next(iter(self._steps)))    # least recently used

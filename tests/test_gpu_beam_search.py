@@ -153,3 +153,14 @@ def test_beam_search_by_the_command_line(tmp_path):
     out = json.loads([line for line in proc.stdout.splitlines() if line.startswith("{")][0])
     last = lambda tokens: plain_gpt.forward_logits(tokens, tensors, cfg.n_layer, cfg.n_head, cfg.layer_norm_epsilon)[-1]  # noqa: E731
     check(out["beams"], plain_beam.search(last, prompt, 3, 6))
+
+
+def test_a_search_of_few_tokens_keeps_the_captured_step():
+    """Searches of too few tokens to be captured replay a step that is, and leave it to those that follow."""
+    engine, last, tokens, vocab = engine_for("A", "float32")
+    graphs = []
+    for made in (8, 5, 8):
+        prompt = tokens(14, 90 + made)
+        check(engine.beam_search([prompt], BeamParams(beams=3, max_tokens=made))[0], plain_beam.search(last, prompt, 3, made))
+        graphs.append([s.graph for s in engine._beam_search._steps.values()])
+    assert len(graphs[0]) == 1 and graphs[0] == graphs[1] == graphs[2]
