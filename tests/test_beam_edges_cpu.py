@@ -7,14 +7,26 @@ import math
 import pytest
 import torch
 
+import fakilorn_cases
 import plain_beam
+from beam_torch_ops import BeamTorchOps
 from test_beam_cpu import ops  # noqa: F401
 from test_beam_search_cpu import engine_for
 
-from mini_gpt_inference_b200 import BeamParams
+from mini_gpt_inference_b200 import BeamParams, EngineConfig, FakilornConfig, LLMEngine
+from mini_gpt_inference_b200.engine.build import load_model
 from mini_gpt_inference_b200.engine.runner import StepError
 from mini_gpt_inference_b200.kernels.library import KernelLibraryError
 from mini_gpt_inference_b200.kernels.ops import BeamChoice
+
+
+def fakilorn_engine(which, device, ops=None):
+    raw = fakilorn_cases.config(which)
+    tensors = fakilorn_cases.random_weights(raw, 7, torch.float32)
+    engine = LLMEngine(load_model(config=FakilornConfig.from_dict(raw), tensors=tensors, dtype="float32", device=device),
+                       EngineConfig(block_size=8, num_blocks=256, max_batch_size=12, max_num_batched_tokens=16, dtype="float32", device=device),
+                       ops=ops)
+    return engine, lambda tokens: fakilorn_cases.plain_logits(raw, tensors, tokens)[-1], lambda n, seed: fakilorn_cases.tokens_for(raw, n, seed)
 
 
 @pytest.mark.parametrize("penalty", [-16.0, -3.5, 16.0])
@@ -96,3 +108,17 @@ def test_outputs_of_a_choice_that_lie_in_its_inputs_are_refused(ops):  # noqa: F
             ops.beam_select(torch.zeros(2 * in_beams, 50), torch.zeros(2, in_beams), beams, ended=ended, lengths=lengths, end_token=1, out=out)
     with pytest.raises(AssertionError, match="mg_beam_select was reached"):      # in place: as the search calls it
         call(3, 3, lambda g, n: dict(scores=g["scores"], ended=g["ended"], lengths=g["lengths"]))
+
+
+@pytest.mark.parametrize("which", ["A", "B", "C", "D"])
+def test_beam_search_of_the_architecture_with_a_blending_chain(which):
+    """Fakilorn: values blended from layer to layer, experts, a state of token pairs."""
+    engine, last, tokens = fakilorn_engine(which, "cpu", BeamTorchOps())
+    prompts = [tokens(n, 30 + n) for n in (5, 17)]
+    found = engine.beam_search(prompts, BeamParams(beams=4, max_tokens=6))
+    for prompt, mine in zip(prompts, found):
+        want = plain_beam.search(last, prompt, 4, 6)
+        assert [h["token_ids"] for h in mine] == [ids for ids, _, _ in want]
+        for h, (_, logprob, _) in zip(mine, want):
+            assert h["logprob"] == pytest.approx(logprob, abs=2e-4)
+    engine.runner.manager.check()
