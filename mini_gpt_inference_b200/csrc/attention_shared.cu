@@ -4,7 +4,11 @@
 // A row's result is the softmax average over the keys 0 .. its position, as in the other attention kernels; what differs is
 // how often the keys are read.  Where every row reads all of its keys, a prompt of P tokens continued B times is read B
 // times.  Here the keys are cut into ranges of two kinds: those of the P tokens that a group's rows share, read once for
-// all (row, head) pairs of the group and key/value head, and those behind them, read for their own row.  A range leaves
+// the (row, head) pairs of the group and key/value head that a CTA takes, and those behind them, read for their own row.
+// (A CTA takes 256 pairs on tcgen05; on the warp-level tensor cores 32, at heads beyond 64 features 16, beyond 128 eight; in 32
+// bits 16.  A group of more pairs has more CTAs, and each of them reads the shared keys.  32 rows of 2,000 shared tokens in a
+// captured step, us, against every row reading its own: heads of 256, 8/2 (16 CTAs of eight pairs) 29 and 40, 8/8 (four) 39
+// and 89; 8 x 8 rows of 1,021, 8/8 heads of 64 13 and 20, of 96 20 and 166, in 32 bits 55 and 68.)  A range leaves
 // per (row, head) its unnormalised average acc, its maximum m (of the scores times log2 e) and its sum l, and a second
 // kernel joins them:  M = max m_i,  out = sum 2^(m_i - M) acc_i / sum 2^(m_i - M) l_i.
 //
@@ -1198,16 +1202,19 @@ struct Cut {
 Cut cut(int n_groups, int max_rows, int max_tokens, int max_behind, int n, int n_head, int n_kv_head, int head_dim, int page_tokens,
         int kind) {
     Cut c;
-    // So few keys that reading them once a row costs less than a second kernel.  (8 heads of 64, two kernels / one, us: 4 rows of 94
-    // keys 6.5 / 4.8, of 256 7.0 / 6.4, of 512 7.8 / 9.1; 64 rows of 256 11.3 / 8.1, of 1,024 14.3 / 19.0; 256 rows of 128
-    // 25.7 / 19.2, of 256 26.3 / 26.0, of 512 39.8 / 38.3; 512 rows of 128 36.9 / 34.5, of 190 38.2 / 41.3.)
+    // So few keys that reading them once a row costs less than a second kernel in bfloat16.  (8 heads of 64, three quarters of the keys
+    // shared, in a captured step, two kernels / one, us: 4 rows of 94 keys 6.1 / 4.5, of 256 6.0 / 6.0, of 512 7.0 / 9.0; 64 rows of
+    // 128 8.1 / 6.8, of 256 8.2 / 9.6, of 1,024 15.2 / 25.7; 256 rows of 128 22.6 / 15.3, of 256 23.5 / 22.4, of 512 29.2 / 33.6; 512
+    // rows of 128 33.4 / 27.5, of 190 34.8 / 33.6, of 256 36.7 / 39.2.  In 32 bits, where one launch costs time: 4 rows of 94 11.2 / 13.2,
+    // of 256 11.8 / 26.0; 64 rows of 128 16.8 / 20.9; 256 rows of 128 64 / 69.)
     const long long keys = n_groups == 0 ? max_behind : (long long)max_tokens + max_behind;
     c.direct = keys <= DIRECT_KEYS / 2 || (keys <= DIRECT_KEYS && (n_groups == 0 || n <= DIRECT_ROWS));
     if (c.direct) n_groups = 0;
     const int share = n_head / n_kv_head, pairs = n_groups > 0 ? (max_rows < n ? max_rows : n) * share : share;
     c.mma = kind == BF16_ALIGNED && head_dim % 8 == 0;
-    // tcgen05 from 32 pairs on.  (mma.sync / tcgen05, us, 2,000 shared tokens: 8 heads of 64, 16 pairs 18.1 / 19.3, 32 22.2 / 16.0, 128
-    // 32.0 / 22.9; 32/8 heads of 128, 16 pairs 23.5 / 19.1 and with 300 tokens 12.3 / 14.6, 32 32.1 / 21.5, 512 76 / 36.5.)
+    // tcgen05 from 32 pairs on.  (mma.sync / tcgen05, us in a captured step, 2,000 shared tokens: 8 heads of 64, 16 pairs 14.6 / 15.6, 32
+    // 23.2 / 16.3 and with 300 tokens 11.4 / 10.1, 128 32.3 / 21.9; 32/8 heads of 128, 16 pairs 20.8 / 17.0 and with 300 tokens
+    // 9.3 / 11.1, 32 20.5 / 17.4 and with 300 tokens 10.0 / 11.6, 512 75.9 / 33.6.)
     c.tc = n_groups > 0 && kind == BF16_ALIGNED && (head_dim == 64 || head_dim == 128) && pairs >= TC_LEAST_PAIRS && page_tokens % 8 == 0 &&
            (page_tokens < TC_KEYS ? TC_KEYS % page_tokens == 0 : page_tokens % TC_KEYS == 0) && max_tokens >= TC_KEYS;
     const int most_tiles = head_dim <= 64 ? 4 : head_dim <= 128 ? 2 : 1;      // what the registers hold
@@ -1217,7 +1224,9 @@ Cut cut(int n_groups, int max_rows, int max_tokens, int max_behind, int n, int n
     c.shared_least = c.tc ? TC_KEYS : BLOCK_KEYS;
     const long long shared_ctas = (long long)n_groups * c.row_tiles * n_kv_head, own_ctas = (long long)n * n_kv_head;
     const int most_shared = ceil_div(max_tokens > 0 ? max_tokens : 1, c.shared_least), most_own = ceil_div(max_behind, OWN_LEAST);
-    // (CTAs of each kind; 8 x 8 rows of about 1,021 shared tokens, 8 heads of 64: 14.2 us with two an SM, 16.9 with four, 15.3 with one)
+    // (CTAs of each kind; us in a captured step with one, two and four an SM: 8 x 8 rows of about 1,021 shared tokens, 8 heads of 64
+    // 11.7, 12.9, 14.7; 4 rows of 2,000 10.2, 12.2, 12.1; 8 x 8 rows of 1,000, 32/8 heads of 128 26.7, 26.8, 27.1; 2 x 5 rows of 509, 12
+    // heads of 64 in 32 bits 19.3, 14.8, 14.8)
     const long long want = 148 * 2;
     long long x = shared_ctas > 0 ? (want + shared_ctas - 1) / shared_ctas : 1;
     if (c.tc) {
