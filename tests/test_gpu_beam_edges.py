@@ -10,7 +10,7 @@ import pytest
 import torch
 
 import plain_beam
-from test_gpu_beam import BF16, F32, check_choice, i32, run_attention, shared_case
+from test_gpu_beam import BF16, F32, check_attention, check_choice, i32, run_attention, shared_case
 
 pytestmark = pytest.mark.gpu
 
@@ -154,6 +154,49 @@ def test_attention_shared_holds_weights_as_paged_attention_does(ops, heads, page
         tol = (2.0 ** -16 + 20 * math.sqrt(D) * 2.0 ** -24) * size + 2.0 ** -8 * want.abs() + 1e-6
         bad = (out[r].double().cpu().reshape(H, D) - want).abs() / tol
         assert (bad <= 1).all(), (r, float(bad.max()))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("groups", [[(20, [1 + i % 3 for i in range(64)])] * 64, [(300, [1 + i % 5 for i in range(32)])] * 32])
+def test_attention_shared_of_some_thousand_rows(ops, dtype, groups):
+    case = shared_case(groups, [7], (4, 2, 16), 16, dtype, seed=64, pad=3)
+    out = run_attention(ops, case)
+    check_attention(case, out, dtype)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_attention_shared_of_one_request_in_several_rows(ops, kernel):
+    """Rows of the same request, at the same position and at others: each sees the keys up to its own."""
+    dtype, heads, groups = KERNELS[kernel]
+    case = shared_case(groups, [40], heads, 16, dtype, seed=65)
+    for r, of, n in ((1, 0, case.k[0].shape[1]), (2, 0, case.k[0].shape[1] - 4)):
+        if r < len(groups[0][1]):
+            case.ctx.token_request[r], case.ctx.positions[r] = int(case.ctx.token_request[of]), n - 1
+            case.k[r], case.v[r] = case.k[of][:, :n], case.v[of][:, :n]
+    assert not check_numbers(case, run_attention(ops, case), dtype)
+
+
+def test_attention_and_choice_on_two_streams_at_once(ops):
+    """Calls that overlap on the GPU share nothing."""
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    cases = [shared_case([(900, [90, 1, 70] * 14)], [400], (8, 8, 64), 16, BF16, seed=66 + i) for i in range(2)]
+    gen = torch.Generator().manual_seed(8)
+    logits, scores = [torch.randn(32, 9000, generator=gen) for _ in range(2)], -3 * torch.rand(4, 8, generator=gen)
+    on_device, first, outs = [x.cuda() for x in logits], scores.cuda(), [[], []]
+    torch.cuda.synchronize()
+    for _ in range(6):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                outs[i].append((run_attention(ops, cases[i]), ops.beam_select(on_device[i], first, 8)))
+    torch.cuda.synchronize()
+    ops.check_status()
+    for case, mine, x in zip(cases, outs, logits):
+        check_attention(case, mine[0][0], BF16)
+        check_choice(mine[0][1], plain_beam.beam_select(x, scores, 8), 4, 8)
+        for out, choice in mine[1:]:
+            assert torch.equal(out, mine[0][0])
+            for name in ("tokens", "parents", "scores", "ranks"):
+                assert torch.equal(getattr(choice, name), getattr(mine[0][1], name))
 
 
 # ---- the choice of the next beams ------------------------------------------------------------------------
